@@ -1,0 +1,451 @@
+"""The operators around the quantised KV cache, as measurable cases: attention over a prompt's own keys and values
+(`prompt_attention`), the weight that cached keys receive (`key_weights`), and the eviction of the others (`evict_keys`).
+
+With `own` false, `run()` computes them from elementary torch operations in 32 bits; with `own` true it calls the
+package. `exact()` gives the results in 64 bits, one sequence at a time.
+
+A batch's sequences have lengths of their own where `ragged` is true, drawn from the number `lens`.
+"""
+import math
+import random
+import sys
+
+import torch
+
+own = False
+
+DEVICE = "cuda"
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def prompt(name, type, nq, nkv, hs, seqs, tokens, cached=0, ragged=False, lens=0, causal=True):
+    """`seqs` prompts of up to `tokens` tokens after up to `cached` earlier ones whose keys and values are at hand."""
+    return dict(name=name, op="prompt", type=type, nq=nq, nkv=nkv, hs=hs, seqs=seqs, tokens=tokens, cached=cached,
+                ragged=ragged, lens=lens, causal=causal)
+
+
+def weights(name, key, nq, nkv, hs, seqs, tokens, context, bs=16, ragged=False, lens=0, decay=1.0):
+    """`tokens` query tokens of each sequence over a context of up to `context` cached keys; decay 0: no earlier weights."""
+    return dict(name=name, op="weights", key=key, nq=nq, nkv=nkv, hs=hs, seqs=seqs, tokens=tokens, context=context,
+                bs=bs, ragged=ragged, lens=lens, decay=decay)
+
+
+def evict(name, key, nkv, hs, seqs, context, budget, sinks, recent, bs=16, ragged=False, lens=0):
+    """The `budget` keys of most weight out of up to `context`, the first `sinks` and the last `recent` among them."""
+    return dict(name=name, op="evict", key=key, nkv=nkv, hs=hs, seqs=seqs, context=context, budget=budget, sinks=sinks,
+                recent=recent, bs=bs, ragged=ragged, lens=lens)
+
+
+def listed():
+    return [
+        # a short question: the smallest prompt, set by latency
+        prompt("prompt-33", "bf16", 32, 8, 128, 1, 33),
+        # new prompts of different lengths in one batch
+        prompt("prompts-2k-ragged", "bf16", 32, 8, 128, 8, 2048, ragged=True, lens=8),
+        # a long document in one call: the largest
+        prompt("prompt-16k", "bf16", 32, 8, 128, 1, 16384),
+        # a prompt of a model with heads of 256
+        prompt("prompt-4k-h256", "bf16", 24, 4, 256, 1, 4096),
+        # the next turns of four conversations in a small fp16 model
+        prompt("turns-h64-fp16", "fp16", 32, 8, 64, 4, 509, cached=4096, ragged=True, lens=3),
+        # one new token of one sequence over a long context that is not quantised
+        prompt("token-64k", "bf16", 64, 8, 128, 1, 1, cached=65536),
+        # the weights of one decode step over a long document, added to those of the steps before
+        weights("weights-step-128k", "int4", 24, 4, 256, 1, 1, 131072),
+        # the same for a batch of requests of different ages on the k8v4 cache, some with a draft token
+        weights("weights-step-b32", "int8", 24, 4, 256, 32, 2, 32768, ragged=True, lens=4, decay=0.99),
+        # the weights from the last 64 tokens of a prompt, before its cache is cut down
+        weights("weights-window-32k", "int4", 64, 8, 128, 1, 64, 32768, decay=0.0),
+        # a short conversation's cache halved: the smallest eviction
+        evict("evict-1k", "int4", 8, 128, 1, 1100, 512, 4, 32),
+        # a long document's cache cut to an eighth
+        evict("evict-128k", "int4", 4, 256, 1, 131072, 16384, 4, 128),
+        # a batch of requests of different lengths, some shorter than the budget, on the k8v4 cache in 32-token blocks
+        evict("evict-b16", "int8", 8, 128, 16, 16384, 2048, 4, 64, bs=32, ragged=True, lens=6),
+    ]
+
+
+HEADS = {64: ((32, 8), (8, 8)), 128: ((32, 8), (64, 8), (28, 4), (16, 16)), 256: ((24, 4), (32, 2), (16, 4)), 512: ((16, 2),)}
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """A case of the same ranges, with no more work than the largest listed one of its operator."""
+    hs = rng.choice((64, 128, 128, 128, 256, 256, 512))
+    nq, nkv = rng.choice(HEADS[hs])
+    op = rng.choice(("prompt", "prompt", "weights", "evict"))
+    lens, ragged = rng.randrange(10 ** 6), rng.random() < 0.6
+    if op == "prompt":
+        kind = rng.choice(("one", "many", "many", "turn", "token"))
+        seqs = 1 if kind == "one" else _log_int(rng, 1, 16)
+        tokens = 1 if kind == "token" else _log_int(rng, 2, 8192 if kind == "one" else 2048)
+        cached = _log_int(rng, 16, 65536 if kind == "token" else 16384) if kind in ("turn", "token") else 0
+        causal = kind != "many" or rng.random() < 0.7
+        c = prompt("", rng.choice(("bf16", "bf16", "fp16")), nq, nkv, hs, seqs, tokens, cached, ragged, lens, causal)
+        while seqs * nq * c["tokens"] * (c["tokens"] + c["cached"]) > 2e9 or \
+                seqs * (c["tokens"] + c["cached"]) * nkv * hs > 3e8 or work(c)["flops"] > 6e11:
+            c["tokens"] -= c["tokens"] // 4
+            c["cached"] -= c["cached"] // 4
+    elif op == "weights":
+        seqs = rng.choice((1, 1, _log_int(rng, 2, 64)))
+        tokens = rng.choice((1, 1, 2, 4, _log_int(rng, 5, 128)))
+        c = weights("", rng.choice(("int4", "int4", "int8")), nq, nkv, hs, seqs, tokens, _log_int(rng, 128, 262144),
+                    rng.choice((16, 16, 32, 48)), ragged, lens, rng.choice((0.0, 0.9, 1.0)))
+        while seqs * c["context"] * nkv * hs > 2e9 or seqs * nq * tokens * c["context"] > 1e9:
+            c["context"] -= c["context"] // 4
+    else:
+        seqs, context = _log_int(rng, 1, 64), _log_int(rng, 64, 262144)
+        while seqs * context * nkv * hs > 1e9:
+            context -= context // 4
+        budget = max(8, int(context * rng.uniform(0.05, 0.8)))
+        c = evict("", rng.choice(("int4", "int4", "int8")), nkv, hs, seqs, context, budget, rng.choice((0, 1, 4, 7)),
+                  min(budget // 2, rng.choice((0, 8, 33, 128))), rng.choice((16, 16, 32, 48)), ragged, lens)
+    del c["name"]
+    return c
+
+
+# ------------------------------------------------------------------------------------------- shapes of a case
+
+def lengths(case):
+    """(query tokens, keys including theirs) of every sequence."""
+    rng = random.Random(case["lens"])
+
+    def up_to(n):
+        return rng.randint(max(1, n // 8), n) if case["ragged"] and n > 1 else n
+
+    got = []
+    for _ in range(case["seqs"]):
+        if case["op"] == "prompt":
+            q = up_to(case["tokens"])
+            got.append((q, q + (up_to(case["cached"]) if case["cached"] else 0)))
+        elif case["op"] == "weights":
+            q = rng.randint(1, case["tokens"]) if case["ragged"] else case["tokens"]
+            got.append((q, max(q, up_to(case["context"]))))
+        else:
+            got.append((0, up_to(case["context"])))
+    return got
+
+
+def pairs(case):
+    """(query token, key) pairs with the key in sight of the token."""
+    if case["op"] == "prompt" and not case["causal"]:
+        return sum(q * n for q, n in lengths(case))
+    return sum(q * n - q * (q - 1) // 2 for q, n in lengths(case))
+
+
+def work(case):
+    lens, hs, nkv = lengths(case), case["hs"], case["nkv"]
+    tokens, keys = sum(q for q, _ in lens), sum(n for _, n in lens)
+    if case["op"] == "prompt":  # q and out, k and v, the row's log-sum-exp
+        nq = case["nq"]
+        return {"bytes": 4 * tokens * nq * hs + 4 * keys * nkv * hs + 4 * tokens * nq, "flops": 4 * hs * nq * pairs(case)}
+    kb = hs // 2 if case["key"] == "int4" else hs
+    if case["op"] == "weights":  # the key halves of the cells, the queries, the weights (read where there are earlier ones)
+        nq = case["nq"]
+        return {"bytes": keys * nkv * (kb + 4 + (8 if case["decay"] else 4)) + 2 * tokens * nq * hs,
+                "flops": 2 * hs * nq * pairs(case)}
+    kept = sum(min(n, case["budget"]) for _, n in lens)  # the weights; the kept cells in and out, their places and weights
+    return {"bytes": 4 * keys * nkv + kept * nkv * (2 * (kb + hs // 2 + 8) + 8), "flops": keys * nkv}
+
+
+# --------------------------------------------------------------------------------------------------- inputs
+
+def _cu(lens):
+    return torch.tensor([0] + lens, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(DEVICE)
+
+
+def _words(shape, median, gen):
+    """fp32 scale words with a zero point of 6..9 in the low four bits."""
+    s = (torch.randn(shape, generator=gen, device=DEVICE) * 0.2).exp_() * median
+    zp = torch.randint(6, 10, shape, generator=gen, device=DEVICE, dtype=torch.int32)
+    return (s.view(torch.int32) & -16 | zp).view(torch.float32)
+
+
+def _cache(case, blocks, gen):
+    """A byte cache (blocks, KV heads, slots, cell) in the Hadamard domain of keys of unit variance, and its views."""
+    nkv, bs, hs = case["nkv"], case["bs"], case["hs"]
+    int4 = case["key"] == "int4"
+    kb, vb = hs // 2 if int4 else hs, hs // 2
+    kv = torch.randint(0, 256, (blocks, nkv, bs, kb + vb + 8), generator=gen, device=DEVICE, dtype=torch.uint8)
+    words = kv.view(torch.float32)
+    shape, unit = (blocks, nkv, bs), hs ** 0.5  # a key's channels have this deviation once rotated
+    words[..., (kb + 4 + vb) // 4] = _words(shape, unit / 4.6, gen)
+    if int4:
+        words[..., kb // 4] = _words(shape, unit / 4.6, gen)  # (codes uniform over 0..15 deviate by 4.6)
+    else:
+        words[..., kb // 4] = (torch.randn(shape, generator=gen, device=DEVICE) * 0.2).exp_() * (unit / 73)
+    t, w = kv.transpose(1, 2), words.transpose(1, 2)
+    k = t[..., :kb]
+    return dict(kv=kv, k=k if int4 else k.view(torch.int8), v=t[..., kb + 4:kb + 4 + vb], ks=w[..., kb // 4],
+                vs=w[..., (kb + 4 + vb) // 4])
+
+
+def _tables(counts, gen, first=0):
+    """A block table of shuffled physical blocks from `first` on."""
+    pool = torch.randperm(sum(counts), generator=gen, device=DEVICE).to(torch.int32) + first
+    table = torch.zeros((len(counts), max(counts)), dtype=torch.int32, device=DEVICE)
+    at = 0
+    for i, c in enumerate(counts):
+        table[i, :c] = pool[at:at + c]
+        at += c
+    return table
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device=DEVICE).manual_seed(seed)
+    lens = lengths(case)
+    qlens, klens = [q for q, _ in lens], [n for _, n in lens]
+    hs, nkv = case["hs"], case["nkv"]
+    s = dict(case=case, max_q=max(qlens), max_k=max(klens))
+    if case["op"] == "prompt":
+        dtype = TYPES[case["type"]]
+        # logits with a deviation of 3: a few keys take most of a row's weight, as in trained models
+        s["q"] = (torch.randn((sum(qlens), case["nq"], hs), generator=gen, device=DEVICE) * 3).to(dtype)
+        s["k"], s["v"] = (torch.randn((sum(klens), nkv, hs), generator=gen, device=DEVICE).to(dtype) for _ in range(2))
+        s.update(cu_q=_cu(qlens), cu_k=_cu(klens), out=torch.zeros_like(s["q"]),
+                 lse=torch.zeros((sum(qlens), case["nq"]), device=DEVICE))
+        return s
+    bs = case["bs"]
+    counts = [-(-n // bs) for n in klens]
+    s["used"] = torch.tensor(klens, dtype=torch.int32, device=DEVICE)
+    s["table"] = _tables(counts, gen)
+    if case["op"] == "weights":
+        s.update(_cache(case, sum(counts), gen))
+        s["q"] = (torch.randn((sum(qlens), case["nq"], hs), generator=gen, device=DEVICE) * 3 * hs ** 0.5).to(torch.bfloat16)
+        s["cu_q"] = _cu(qlens)
+        s["out"] = torch.zeros((case["seqs"], nkv, s["max_k"]), device=DEVICE)
+        s["previous"] = torch.rand(s["out"].shape, generator=gen, device=DEVICE) / 64 if case["decay"] else None
+        return s
+    # an eviction: room for the kept cells behind those of the sequences
+    new = [-(-min(n, case["budget"]) // bs) for n in klens]
+    s.update(_cache(case, sum(counts) + sum(new), gen))
+    s["new_table"] = _tables(new, gen, sum(counts))
+    s["first_new"] = sum(counts)
+    shape = (case["seqs"], nkv, s["max_k"])
+    w = (torch.randn(shape, generator=gen, device=DEVICE) * 2 - 6).exp_()  # a few keys hold most of the weight,
+    w[torch.rand(shape, generator=gen, device=DEVICE) < 0.1] = 0.0         # and some have never had any
+    s["weights"] = w
+    s["kept"] = torch.full((case["seqs"], nkv, case["budget"]), -1, dtype=torch.int32, device=DEVICE)
+    s["new_weights"] = torch.zeros((case["seqs"], nkv, case["budget"]), device=DEVICE)
+    s["new_used"] = torch.zeros(case["seqs"], dtype=torch.int32, device=DEVICE)
+    return s
+
+
+# ------------------------------------------------------------------------------------------- the plain forms
+
+def _padded(x, cu, width):
+    """Packed rows as (sequences, width, ...): the rows past a sequence's own are copies of others."""
+    at = cu[:-1, None].long() + torch.arange(width, device=DEVICE)
+    return x[at.clamp(max=x.shape[0] - 1)]
+
+
+def _packed(x, cu, rows):
+    """The rows of (sequences, width, ...) that are the sequences' own, one after the other."""
+    t = torch.arange(rows, device=DEVICE)
+    seq = torch.searchsorted(cu, t, right=True) - 1
+    return x[seq, t - cu[seq]]
+
+
+def _sight(qlens, klens, max_q, max_k, causal):
+    """(sequences, query token, key): whether the token sees the key."""
+    i = torch.arange(max_q, device=DEVICE)[None, :, None]
+    j = torch.arange(max_k, device=DEVICE)[None, None, :]
+    qlens, klens = qlens[:, None, None], klens[:, None, None]
+    last = i + klens - qlens if causal else klens - 1
+    return (i < qlens) & (j <= last) & (j < klens)
+
+
+def _softmax(scores, sight):
+    """exp(score - the row's largest) of the keys in sight, with the row's largest and its sum; in place."""
+    scores.masked_fill_(~sight, float("-inf"))
+    top = scores.amax(-1, keepdim=True)
+    scores.sub_(top.masked_fill(top == float("-inf"), 0.0)).exp_()
+    return scores, top, scores.sum(-1, keepdim=True)
+
+
+def _plain_prompt(s):
+    c = s["case"]
+    nq, nkv, hs = c["nq"], c["nkv"], c["hs"]
+    group, rows = nq // nkv, s["q"].shape[0]
+    q = _padded(s["q"], s["cu_q"], s["max_q"]).float()
+    k, v = (_padded(x, s["cu_k"], s["max_k"]).float().permute(0, 2, 1, 3) for x in (s["k"], s["v"]))
+    seqs, max_q = q.shape[:2]
+    q = q.view(seqs, max_q, nkv, group, hs).permute(0, 2, 3, 1, 4).reshape(seqs, nkv, group * max_q, hs)
+    scores = torch.matmul(q * hs ** -0.5, k.transpose(2, 3).contiguous()).view(seqs, nkv, group, max_q, s["max_k"])
+    sight = _sight(s["cu_q"].diff(), s["cu_k"].diff(), max_q, s["max_k"], c["causal"])[:, None, None]
+    p, top, total = _softmax(scores, sight)
+    out = torch.matmul(p.view(seqs, nkv, group * max_q, s["max_k"]), v.contiguous()).view(seqs, nkv, group, max_q, hs)
+    out = torch.where(total > 0, out / total, torch.zeros_like(out))
+    lse = (top + total.log())[..., 0]
+    out = out.permute(0, 3, 1, 2, 4).reshape(seqs, max_q, nq, hs)
+    lse = lse.permute(0, 3, 1, 2).reshape(seqs, max_q, nq)
+    return _packed(out, s["cu_q"], rows).to(s["q"].dtype), _packed(lse, s["cu_q"], rows)
+
+
+def _cells(s, x):
+    """A cache view's entries of every position of every sequence: (sequences, positions, KV heads, ...)."""
+    bs = s["case"]["bs"]
+    pos = torch.arange(s["max_k"], device=DEVICE)
+    return x[s["table"][:, pos // bs].long(), pos % bs]
+
+
+def _values(codes, words):
+    """What codes and scale words stand for, in the words' precision."""
+    if codes.dtype == torch.int8:
+        return codes.to(torch.float32) * words[..., None]
+    bits = words.contiguous().view(torch.int32)
+    zero, scale = (bits & 15).to(torch.float32), (bits & -16).view(torch.float32)
+    codes = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2)
+    return (codes.to(torch.float32) - zero[..., None]) * scale[..., None]
+
+
+def _plain_weights(s):
+    c = s["case"]
+    nq, nkv, hs = c["nq"], c["nkv"], c["hs"]
+    group = nq // nkv
+    k = _values(_cells(s, s["k"]), _cells(s, s["ks"])).permute(0, 2, 3, 1)
+    q = _padded(s["q"], s["cu_q"], s["max_q"]).float()
+    seqs, max_q = q.shape[:2]
+    q = q.view(seqs, max_q, nkv, group, hs).permute(0, 2, 3, 1, 4).reshape(seqs, nkv, group * max_q, hs)
+    scores = torch.matmul(q * hs ** -1.5, k.contiguous()).view(seqs, nkv, group, max_q, s["max_k"])
+    p, _, total = _softmax(scores, _sight(s["cu_q"].diff(), s["used"], max_q, s["max_k"], True)[:, None, None])
+    w = (p / total.masked_fill(total == 0, 1.0)).sum((2, 3))
+    if s["previous"] is not None:
+        w = w + c["decay"] * s["previous"]
+    valid = torch.arange(s["max_k"], device=DEVICE) < s["used"][:, None, None]
+    return torch.where(valid, w, s["out"])
+
+
+def _plain_evict(s):
+    c = s["case"]
+    bs, budget, used = c["bs"], c["budget"], s["used"][:, None, None]
+    pos = torch.arange(s["max_k"], device=DEVICE)
+    w = s["weights"]
+    order = torch.sort(w, dim=-1, descending=True, stable=True).indices
+    rank = torch.where((pos < c["sinks"]) | (pos >= used - c["recent"]), 0, 1).masked_fill(pos >= used, 2).expand(w.shape)
+    order = order.gather(-1, torch.sort(rank.gather(-1, order), dim=-1, stable=True).indices)
+    count = used.clamp(max=budget)
+    first = torch.arange(budget, device=DEVICE)
+    taken = first < count
+    order = torch.nn.functional.pad(order, (0, max(0, budget - s["max_k"])))[..., :budget]
+    kept = order.masked_fill(~taken, s["max_k"]).sort(dim=-1).values
+    at = kept.clamp(max=s["max_k"] - 1)
+    seq = torch.arange(w.shape[0], device=DEVICE)[:, None, None]
+    head = torch.arange(w.shape[1], device=DEVICE)[None, :, None]
+    cells = s["kv"][s["table"][seq, at // bs].long(), head, at % bs]
+    to = s["new_table"][seq, (first // bs).clamp(max=s["new_table"].shape[1] - 1)].long().expand(at.shape)
+    slot = (first % bs).expand(at.shape)
+    # entries past a sequence's count write what is in their place again, the last of its cells (or the cell itself)
+    to = torch.where(taken, to, s["new_table"][seq, (count - 1) // bs].long())
+    slot = torch.where(taken, slot, (count - 1) % bs)
+    last = cells.gather(2, (count - 1).long()[..., None].expand(*at.shape[:2], 1, cells.shape[-1]))
+    s["kv"][to, head, slot] = torch.where(taken[..., None], cells, last)
+    return (count[:, 0, 0].to(torch.int32), torch.where(taken, kept.to(torch.int32), s["kept"]),
+            torch.where(taken, w.gather(-1, at), s["new_weights"]), s["kv"][s["first_new"]:])
+
+
+# ------------------------------------------------------------------------------------------ the package's calls
+
+def _own(s):
+    if "vllm-quantpack_amd" not in sys.path:
+        sys.path.insert(0, "vllm-quantpack_amd")
+    from vllm_quantpack.attention import eviction, key_weights, prompt
+    c = s["case"]
+    if c["op"] == "prompt":
+        prompt.prompt_attention(s["q"], s["k"], s["v"], s["out"], cu_seqlens_q=s["cu_q"], cu_seqlens_k=s["cu_k"],
+                                max_seqlen_q=s["max_q"], max_seqlen_k=s["max_k"], softmax_scale=c["hs"] ** -0.5,
+                                causal=c["causal"], lse=s["lse"])
+        return s["out"], s["lse"]
+    if c["op"] == "weights":
+        return key_weights.key_weights(s["q"], s["k"], s["ks"], s["out"], cu_seqlens_q=s["cu_q"], seqused_k=s["used"],
+                                       block_table=s["table"], max_seqlen_q=s["max_q"], max_seqlen_k=s["max_k"],
+                                       softmax_scale=c["hs"] ** -1.5, previous=s["previous"], decay=c["decay"])
+    new_used, kept, new_weights = eviction.evict_keys(
+        s["k"], s["v"], s["ks"], s["vs"], s["weights"], seqused_k=s["used"], block_table=s["table"],
+        new_block_table=s["new_table"], budget=c["budget"], max_seqlen_k=s["max_k"], sinks=c["sinks"],
+        recent=c["recent"], kept=s["kept"], new_weights=s["new_weights"], new_seqused_k=s["new_used"])
+    # (the cells are moved, not computed: their bytes are whole numbers that have to be the same)
+    return new_used, kept, new_weights, s["kv"][s["first_new"]:]
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return {"prompt": _plain_prompt, "weights": _plain_weights, "evict": _plain_evict}[state["case"]["op"]](state)
+
+
+# ------------------------------------------------------------------------------------------------ in 64 bits
+
+def _exact_probabilities(q, k, scale, causal):
+    """exp(a - max) over its sum of one sequence's heads, a = scale q.k: q (heads, rows, hs), k (heads, keys, hs)."""
+    rows, keys = q.shape[1], k.shape[1]
+    a = torch.bmm(q, k.transpose(1, 2).contiguous()).mul_(scale)
+    if causal:
+        ahead = torch.arange(keys, device=DEVICE)[None, :] > torch.arange(rows, device=DEVICE)[:, None] + (keys - rows)
+        a.masked_fill_(ahead, float("-inf"))
+    lse = torch.logsumexp(a, -1, keepdim=True)
+    return a.sub_(lse).exp_(), lse[..., 0]
+
+
+def _exact_keys(s, i, n, codes, words):
+    bs = s["case"]["bs"]
+    blocks = s["table"][i, :-(-n // bs)].long()
+    codes, words = codes[blocks].flatten(0, 1)[:n], words[blocks].flatten(0, 1)[:n].contiguous()
+    if codes.dtype == torch.int8:
+        return codes.double() * words.double()[..., None]
+    bits = words.view(torch.int32)
+    full = torch.empty((*codes.shape[:-1], 2 * codes.shape[-1]), dtype=torch.float64, device=DEVICE)
+    full[..., 0::2], full[..., 1::2] = (codes % 16).double(), (codes // 16).double()
+    return (full - (bits % 16).double()[..., None]) * (bits - bits % 16).view(torch.float32).double()[..., None]
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    hs, nkv = case["hs"], case["nkv"]
+    if case["op"] == "prompt":
+        group = case["nq"] // nkv
+        out = torch.zeros(s["q"].shape, dtype=torch.float64, device=DEVICE)
+        lse = torch.zeros(s["lse"].shape, dtype=torch.float64, device=DEVICE)
+        tq = tk = 0
+        for q, n in lengths(case):
+            for g in range(nkv):  # a KV head's query heads at a time: 4 GB of probabilities at 16384 tokens and two heads
+                keys, vals = s["k"][tk:tk + n, g].double(), s["v"][tk:tk + n, g].double()
+                for h in range(g * group, (g + 1) * group):
+                    p, lse[tq:tq + q, h] = _exact_probabilities(s["q"][tq:tq + q, h].double()[None], keys[None],
+                                                               hs ** -0.5, case["causal"])
+                    out[tq:tq + q, h] = p[0] @ vals
+            tq, tk = tq + q, tk + n
+        return out, lse
+    if case["op"] == "weights":
+        group = case["nq"] // nkv
+        w = s["out"].double()
+        tq = 0
+        for i, (q, n) in enumerate(lengths(case)):
+            keys = _exact_keys(s, i, n, s["k"], s["ks"])
+            for h in range(case["nq"]):
+                p, _ = _exact_probabilities(s["q"][tq:tq + q, h].double()[None], keys[:, h // group][None], hs ** -1.5, True)
+                w[i, h // group, :n] += p[0].sum(0)
+            if s["previous"] is not None:
+                w[i, :, :n] += case["decay"] * s["previous"][i, :, :n].double()
+            tq += q
+        return w
+    # an eviction: sorted on the host, one (sequence, head) after the other
+    used, kept, new_weights = [], s["kept"].cpu(), s["new_weights"].cpu().double()
+    weights, bs = s["weights"].cpu(), case["bs"]
+    cells = s["kv"].clone()
+    for i, (_, n) in enumerate(lengths(case)):
+        count = min(n, case["budget"])
+        used.append(count)
+        for g in range(nkv):
+            w = weights[i, g, :n].double()
+            w[:case["sinks"]] = math.inf
+            w[max(0, n - case["recent"]):] = math.inf
+            best = torch.from_numpy((-w.numpy()).argsort(kind="stable").copy())[:count].sort().values
+            kept[i, g, :count] = best.to(torch.int32)
+            new_weights[i, g, :count] = weights[i, g, best].double()
+            src, dst = best.to(DEVICE), torch.arange(count, device=DEVICE)
+            cells[s["new_table"][i, dst // bs].long(), g, dst % bs] = s["kv"][s["table"][i, src // bs].long(), g, src % bs]
+    return torch.tensor(used, dtype=torch.int32), kept, new_weights, cells[s["first_new"]:]
