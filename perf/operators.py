@@ -352,17 +352,19 @@ def _plain_evict(s):
 def _own(s):
     if "vllm-quantpack_amd" not in sys.path:
         sys.path.insert(0, "vllm-quantpack_amd")
-    from vllm_quantpack.attention import eviction, key_weights, prompt
     c = s["case"]
     if c["op"] == "prompt":
+        from vllm_quantpack.attention import prompt
         prompt.prompt_attention(s["q"], s["k"], s["v"], s["out"], cu_seqlens_q=s["cu_q"], cu_seqlens_k=s["cu_k"],
                                 max_seqlen_q=s["max_q"], max_seqlen_k=s["max_k"], softmax_scale=c["hs"] ** -0.5,
                                 causal=c["causal"], lse=s["lse"])
         return s["out"], s["lse"]
     if c["op"] == "weights":
+        from vllm_quantpack.attention import key_weights
         return key_weights.key_weights(s["q"], s["k"], s["ks"], s["out"], cu_seqlens_q=s["cu_q"], seqused_k=s["used"],
                                        block_table=s["table"], max_seqlen_q=s["max_q"], max_seqlen_k=s["max_k"],
                                        softmax_scale=c["hs"] ** -1.5, previous=s["previous"], decay=c["decay"])
+    from vllm_quantpack.attention import eviction
     new_used, kept, new_weights = eviction.evict_keys(
         s["k"], s["v"], s["ks"], s["vs"], s["weights"], seqused_k=s["used"], block_table=s["table"],
         new_block_table=s["new_table"], budget=c["budget"], max_seqlen_k=s["max_k"], sinks=c["sinks"],
