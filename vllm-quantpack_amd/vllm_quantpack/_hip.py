@@ -1,4 +1,4 @@
-"""ctypes binding of libquantpack_hip.so (the C ABI declared in include/quantpack.h).
+"""ctypes binding of libquantpack_hip.so (the C ABI declared in include/quantpack.h and include/quantpack_ops.h).
 
 The library is loaded after torch so that its `libamdhip64.so.7` dependency resolves to the HIP runtime torch already
 loaded: device pointers and streams are then shared. There is no fallback: if the library is missing, every call
@@ -6,6 +6,7 @@ raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import struct
@@ -18,7 +19,7 @@ LIB_PATH = os.environ.get("QUANTPACK_HIP_LIB") or os.path.join(os.path.dirname(o
 
 QP_OK, QP_ERR_INVALID, QP_ERR_UNSUPPORTED = 0, -1, -2
 CODES_INT4, CODES_INT8 = 0, 1
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_F16 = 0, 1, 2
 DECODE_TILE = 32          # QP_DECODE_TILE: split-KV segments are multiples of this many keys
 DECODE_MAX_QUERY = 4      # QP_DECODE_MAX_QUERY
 
@@ -77,6 +78,16 @@ class AttentionArgs(Structure):
 class StoreArgs(Structure):
     _fields_ = [("key", c_void_p), ("key_stride", I64x2), ("value", c_void_p), ("value_stride", I64x2),
                 ("slot_mapping", c_void_p), ("num_tokens", c_int32), ("rht_signs", c_void_p)]
+
+
+class PromptArgs(Structure):
+    _fields_ = [("query", c_void_p), ("query_stride", I64x2), ("key", c_void_p), ("key_stride", I64x2),
+                ("value", c_void_p), ("value_stride", I64x2), ("cu_seqlens_q", c_void_p), ("cu_seqlens_k", c_void_p),
+                ("num_seqs", c_int32), ("num_tokens", c_int32), ("num_keys", c_int32), ("num_q_heads", c_int32),
+                ("num_kv_heads", c_int32), ("head_size", c_int32), ("dtype", c_int32), ("max_seqlen_k", c_int32),
+                ("num_splits", c_int32), ("causal", c_int32), ("softmax_scale", c_float), ("out", c_void_p),
+                ("out_stride", I64x2), ("lse", c_void_p), ("lse_stride", I64x2), ("workspace", c_void_p),
+                ("workspace_bytes", c_int64)]
 
 
 _CODES = {c_void_p: "Q", c_int64: "q", c_int32: "i", c_float: "f"}
@@ -143,6 +154,12 @@ SIGNATURES = {
     "qp_version": (c_char_p, []),
 }
 
+# Every entry point of include/quantpack_ops.h.
+OPS_SIGNATURES = {
+    "qp_prompt": (c_int32, [POINTER(PromptArgs), c_void_p]),
+    "qp_prompt_workspace_size": (c_int64, [POINTER(PromptArgs)]),
+}
+
 _lib = None
 
 
@@ -158,7 +175,7 @@ def lib():
             raise HipLibraryMissing(f"{LIB_PATH} is missing: build it with `python vllm-quantpack_amd/build.py` "
                                     "(this package has no CPU or Triton fallback)")
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (SIGNATURES | OPS_SIGNATURES).items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
@@ -185,6 +202,25 @@ def stream_of(t: torch.Tensor):
     if _raw_stream is not None and t.is_cuda:
         return c_void_p(_raw_stream(t.get_device()))
     return c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """A context in which t's device is the current one: a launch goes to the current device, whatever its stream."""
+    index = t.get_device()
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def same_device(what: str, first: torch.Tensor, **tensors) -> None:
+    """ValueError unless first is on a GPU and every other tensor (None: absent) on the same one."""
+    if not first.is_cuda:
+        raise ValueError(f"{what}: tensors must be on a GPU, got {first.device}")
+    index = first.get_device()
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: {name} is on {t.device}, not on {first.device}")
 
 
 def ptr(t):
