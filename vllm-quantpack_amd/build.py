@@ -39,6 +39,7 @@ EXTRA = {"qp_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "qp_prefill_dual.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "qp_prefill_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "qp_prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "qp_key_weights.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          # the one atomic (a chunk claim by lane 0) needs no wave-level reduction around it
          "qp_decode.hip": ["-fno-honor-nans", "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]}
 

@@ -90,6 +90,25 @@ class PromptArgs(Structure):
                 ("workspace_bytes", c_int64)]
 
 
+class KeyWeightsArgs(Structure):
+    _fields_ = [("key", CacheHalf), ("num_blocks", c_int32), ("block_size", c_int32), ("num_kv_heads", c_int32),
+                ("head_size", c_int32), ("query", c_void_p), ("query_stride", I64x2), ("cu_seqlens_q", c_void_p),
+                ("seqused_k", c_void_p), ("block_table", c_void_p), ("block_table_stride", c_int64),
+                ("max_blocks", c_int32), ("num_seqs", c_int32), ("num_tokens", c_int32), ("num_q_heads", c_int32),
+                ("max_query_len", c_int32), ("max_seqlen_k", c_int32), ("softmax_scale", c_float), ("decay", c_float),
+                ("query_signs", c_void_p), ("previous", c_void_p), ("previous_stride", I64x2), ("out", c_void_p),
+                ("out_stride", I64x2), ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
+class EvictArgs(Structure):
+    _fields_ = [("weights", c_void_p), ("weights_stride", I64x2), ("seqused_k", c_void_p), ("block_table", c_void_p),
+                ("block_table_stride", c_int64), ("new_block_table", c_void_p), ("new_block_table_stride", c_int64),
+                ("max_blocks", c_int32), ("new_max_blocks", c_int32), ("num_seqs", c_int32), ("max_seqlen_k", c_int32),
+                ("budget", c_int32), ("sinks", c_int32), ("recent", c_int32), ("kept", c_void_p),
+                ("kept_stride", I64x2), ("new_weights", c_void_p), ("new_weights_stride", I64x2),
+                ("new_seqused_k", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
 _CODES = {c_void_p: "Q", c_int64: "q", c_int32: "i", c_float: "f"}
 
 
@@ -158,6 +177,10 @@ SIGNATURES = {
 OPS_SIGNATURES = {
     "qp_prompt": (c_int32, [POINTER(PromptArgs), c_void_p]),
     "qp_prompt_workspace_size": (c_int64, [POINTER(PromptArgs)]),
+    "qp_key_weights": (c_int32, [POINTER(KeyWeightsArgs), c_void_p]),
+    "qp_key_weights_workspace_size": (c_int64, [POINTER(KeyWeightsArgs)]),
+    "qp_evict": (c_int32, [POINTER(PagedCache), POINTER(EvictArgs), c_void_p]),
+    "qp_evict_workspace_size": (c_int64, [POINTER(PagedCache), POINTER(EvictArgs)]),
 }
 
 _lib = None
