@@ -41,36 +41,7 @@ constexpr float kPromptNone = -1e30f;  // a row's maximum before it has seen a k
 // A row's maximum m is raised when a score exceeds it by more than this (log2 units): probabilities stay below 2^8, well
 // within fp16, whose smallest normal number is then 2^-22 of the largest probability.
 constexpr float kPromptHeadroom = 8.f;
-
-template <int HS_, bool F16_>
-struct PromptShape {
-  static constexpr int HS = HS_;
-  static constexpr bool F16 = F16_;
-  static constexpr int kWaves = HS <= 128 ? 8 : 4;   // two waves per SIMD, or one where a row tile takes over 256 registers
-  // Waves that share a row tile, each with its part of the channels of q, K, V and the accumulators. At head 512 (where
-  // they would take 384 registers) two: each makes the scores of its channels, and the two parts are added through LDS.
-  static constexpr int kParts = HS == 512 ? 2 : 1;
-  static constexpr int kChannels = HS / kParts;
-  static constexpr int kThreads = kWaves * 64;
-  static constexpr int kRt = 1;                      // 32-row tiles per wave
-  static constexpr int kRows = kWaves / kParts * kRt * 32;
-  static constexpr int kKeys = HS == 512 ? 32 : 64;  // keys per tile
-  static constexpr int kStages = HS <= 128 ? 3 : 2;
-  static constexpr int kU = HS / 8;                  // 16-byte units of a row
-  static constexpr int kHalf = kKeys * HS * 2;       // bytes of a tile's K (and of its V)
-  static constexpr int kStage = 2 * kHalf;
-  static constexpr int kScores = kStages * kStage;   // parts of the scores, 4 KiB per wave; or the word of a vote
-  static constexpr int kLds = kScores + (kParts > 1 ? kWaves * 4096 : 16);
-  static constexpr int kCopies = kHalf / 1024 / kWaves;  // 1 KiB copies of a wave, K and V each
-  static_assert(kHalf % (1024 * kWaves) == 0 && kLds <= 160 * 1024, "LDS");
-  // Position of unit c in row r of a K tile: 16 rows' reads of one unit hit every bank of the LDS once.
-  static __host__ __device__ constexpr int k_swz(int r, int c) { return HS == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15); }
-  // The same in a V tile, in blocks of four units (32 channels, what a transposing read takes of a row): the four rows of
-  // a 16-lane group hit different banks. At head 64 a row has two blocks, and two rows every bank.
-  static __host__ __device__ constexpr int v_swz(int r, int c) {
-    return HS == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2);
-  }
-};
+constexpr int kPromptWideRows = 64;       // rows of a workgroup at head 512
 
 template <bool F16>
 __device__ __forceinline__ f32x16_t mfma_prompt(u32x4_t a, u32x4_t b, f32x16_t c) {
@@ -103,349 +74,624 @@ __device__ __forceinline__ float other_half_max(float v) {
   return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 
-template <class Sh>
-__global__ __launch_bounds__(Sh::kThreads) void prompt_kernel(const PromptParams p) {
-  constexpr int HS = Sh::HS, KT = Sh::kKeys, RT = Sh::kRt, U = Sh::kU;
-  constexpr bool F16 = Sh::F16;
-  constexpr int kParts = Sh::kParts, kHc = Sh::kChannels;
-  constexpr int kCs = kHc / 16, kCt = kHc / 32, kSubs = KT / 32;
-  static_assert(kParts == 1 || (RT == 1 && kSubs == 1 && kParts == 2), "parts of the scores");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[Sh::kLds];
+// log2 of the XCDs that share a (KV head, split) pair's row blocks: 8 over the largest power of two in the pairs.
+__host__ __device__ __forceinline__ uint32_t prompt_share(uint32_t pairs) {
+  return (pairs & 7) == 0 ? 0 : (pairs & 3) == 0 ? 1 : (pairs & 1) == 0 ? 2 : 3;
+}
 
-  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
-  const int col = lane & 31, h = lane >> 5;
-  const int part = w % kParts;
-  const int blk = (int)gridDim.x - 1 - (int)blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
-  const int G = p.num_q_heads / p.num_kv_heads;
-  // row block -> sequence: sequence s's rows own blocks [cu_q[s] G / kRows + s, ...)
-  int lo = 0, hi = p.num_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((int)(((int64_t)p.cu_q[mid] * G) / Sh::kRows) + mid <= blk) lo = mid;
-    else hi = mid - 1;
+// ------------------------------------------------------------------------------------ what the kernels share
+
+// A workgroup's part of the work: rows r0 .. of sequence `seq`'s (token, query head) rows of KV head kvh, keys [kb, ke) of
+// its n. False: none.
+struct PromptBlock {
+  int kvh, q0, qlen, k0, n, nrows, r0, kb, ke, split;
+};
+
+template <int ROWS>
+__device__ __forceinline__ bool prompt_block(const PromptParams &p, PromptBlock &b) {
+  // Workgroups go to the 8 XCDs in turn: 2^share of them take the row blocks of the same (KV head, split) pairs, so that
+  // the blocks that share keys share as few L2s as balance allows. Later blocks, which see more keys, come first.
+  const uint32_t lin = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+  const uint32_t pairs = gridDim.y * gridDim.z, share = prompt_share(pairs), per = gridDim.x >> share;
+  const uint32_t xcd = lin & 7, turn = (lin >> 3) / per;
+  const uint32_t pair = (xcd >> share) * ((pairs << share) >> 3) + turn;
+  const int blk = (int)(gridDim.x - 1 - ((((lin >> 3) - turn * per) << share) + (xcd & ((1u << share) - 1))));
+  b.kvh = (int)(pair % gridDim.y);
+  b.split = (int)(pair / gridDim.y);
+  const int G = p.num_q_heads / p.num_kv_heads, lane = threadIdx.x & 63;
+  // row block -> sequence: sequence s's rows own blocks [cu_q[s] G / ROWS + s, ...). 63 sequences are looked at in one go
+  int seq = -1, q1 = 0, k1 = 0;
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 63) {
+    const int i = min(s0 + lane, p.num_seqs);
+    const int cq = p.cu_q[i], ck = p.cu_k[i];
+    const uint64_t before =
+        __ballot(s0 + lane < p.num_seqs && lane < 63 && (int)(((int64_t)cq * G) / ROWS) + s0 + lane <= blk);
+    if (!before) break;
+    const int at = 63 - __builtin_clzll(before);
+    seq = s0 + at;
+    b.q0 = __builtin_amdgcn_readlane(cq, at);
+    q1 = __builtin_amdgcn_readlane(cq, at + 1);
+    b.k0 = __builtin_amdgcn_readlane(ck, at);
+    k1 = __builtin_amdgcn_readlane(ck, at + 1);
+    if (at < 62) break;
   }
-  const int seq = lo;
-  const int q0 = max(0, p.cu_q[seq]), qlen = min(p.cu_q[seq + 1], p.num_tokens) - q0;
-  const int k0 = max(0, p.cu_k[seq]), n = max(0, min(p.cu_k[seq + 1], p.num_keys) - k0);
-  const int nrows = qlen * G;
-  const int r0 = (blk - (int)(((int64_t)q0 * G) / Sh::kRows) - seq) * Sh::kRows;
-  if (r0 < 0 || r0 >= nrows) return;
-  // the last position that a token sees, first and last token of the block
-  auto last_pos = [&](int tok) { return p.causal ? n - qlen + tok : n - 1; };
-  const int kend = max(0, min(n, last_pos((min(nrows, r0 + Sh::kRows) - 1) / G) + 1));
-  const int S = p.num_splits;
-  const int seg = segment_keys(n, S, p.min_keys);
-  const int64_t kb64 = (int64_t)split * seg;
-  if (S > 1 && kb64 >= n) return;  // an empty segment: the merge does not read it
-  const int kb = (int)kb64;
-  const int ke = uniform(min((int64_t)kend, kb64 + seg));
+  if (seq < 0) return false;
+  b.q0 = max(0, b.q0);
+  b.k0 = max(0, b.k0);
+  b.qlen = min(q1, p.num_tokens) - b.q0;
+  b.n = max(0, min(k1, p.num_keys) - b.k0);
+  b.nrows = b.qlen * G;
+  b.r0 = (blk - (int)(((int64_t)b.q0 * G) / ROWS) - seq) * ROWS;
+  if (b.r0 < 0 || b.r0 >= b.nrows) return false;
+  const int last = p.causal ? b.n - b.qlen + (min(b.nrows, b.r0 + ROWS) - 1) / G : b.n - 1;
+  const int seg = segment_keys(b.n, p.num_splits, p.min_keys);
+  const int64_t kb = (int64_t)b.split * seg;
+  if (p.num_splits > 1 && kb >= b.n) return false;  // an empty segment: the merge does not read it
+  b.kb = (int)kb;
+  b.ke = uniform((int)min((int64_t)max(0, min(b.n, last + 1)), kb + seg));
+  return true;
+}
 
-  // ---- the wave's rows: lane row col of tile rt -> (token rr / G, query head rr % G)
-  const int wrow = r0 + 32 * RT * (w / kParts);
-  const bool active = wrow < nrows;
-  int row_pos[RT], tok[RT], jh[RT];
-  u32x4_t qop[RT][kCs];
+// The V^T operand's lane offset in a tile of rows of HS channels: A row 8 q + 4 hh + j of channel tile ct is channel
+// 32 ct + 16 hh + 4 q + j, so that a lane's accumulators are 16 consecutive channels. A 16-lane group reads four keys' rows,
+// lanes 4 k .. 4 k + 3 the four 4-channel chunks 16 (c & 1) + 4 (c >> 1) of key k (8 channels further in the upper group),
+// and gets them transposed: a lane four keys of its channel.
+__device__ __forceinline__ int v_row(int lane) { return 4 * (lane >> 5) + ((lane >> 2) & 3); }
+__device__ __forceinline__ int v_channel(int lane) {
+  return 16 * (lane & 1) + 4 * ((lane >> 1) & 1) + 8 * ((lane >> 4) & 1);
+}
+
+// The operand's 8 keys of a channel: keys 4 h .. and 8 + 4 h .. of 16 (h the wave half), as the packed probabilities lie.
+template <int HS>
+__device__ __forceinline__ u32x4_t v_operand(const uint8_t *at) {
+  u32x4_t r;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int rr = wrow + 32 * rt + col;
-    const bool valid = rr < nrows;
-    tok[rt] = valid ? rr / G : -1;
-    jh[rt] = valid ? rr - tok[rt] * G : 0;
-    row_pos[rt] = valid ? last_pos(tok[rt]) : -1;
-    const uint16_t *src = p.q + (int64_t)(q0 + max(0, tok[rt])) * p.qs0 + (int64_t)(kvh * G + jh[rt]) * p.qs1 + kHc * part + 8 * h;
-#pragma unroll
-    for (int cs = 0; cs < kCs; ++cs)
-      qop[rt][cs] = valid ? *reinterpret_cast<const u32x4_t *>(src + 16 * cs) : u32x4_t{0u, 0u, 0u, 0u};
+  for (int eight = 0; eight < 2; ++eight) {
+    const i16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) i16x4_t *)(const __attribute__((address_space(3))) uint8_t *)(at + eight * 16 * HS));
+    const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
+    r[2 * eight] = y[0];
+    r[2 * eight + 1] = y[1];
   }
-  f32x16_t acc[RT][kCt];
-  float m[RT], l[RT];
+  return r;
+}
+
+// Infinities and NaN in the values of keys that some row of a wave does not see: such a row's probability is 0, and the
+// MFMA would make NaN of the product. A wave that meets them takes zeros in their place, and adds the value itself to the
+// rows that see the key afterwards (any probability is above 0).
+template <bool F16>
+struct Odd {
+  static constexpr uint32_t kInf = F16 ? 0x7C00u : 0x7F80u;
+  static __device__ __forceinline__ u32x4_t without(u32x4_t x) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = kPromptNone;
-    l[rt] = 0.f;
-#pragma unroll
-    for (int ct = 0; ct < kCt; ++ct) acc[rt][ct] = f32x16_t{};
+    for (int j = 0; j < 4; ++j) {
+      if ((x[j] & kInf) == kInf) x[j] &= 0xFFFF0000u;
+      if ((x[j] & (kInf << 16)) == kInf << 16) x[j] &= 0xFFFFu;
+    }
+    return x;
   }
-
-  const int ntiles = ke > kb ? (ke - kb + KT - 1) / KT : 0;
-  if (ntiles > 0) {
-    // tiles whose keys every row of the block (of the wave) sees, and tiles that some row of the wave sees
-    auto plain_tiles = [&](int row) { return max(0, min(last_pos(row / G) + 1, ke) - kb) / KT; };
-    // (waves that share scores meet at barriers in a tile, so there the block goes by its own bounds)
-    const int bplain = uniform(plain_tiles(r0));
-    const int wlast = last_pos((min(nrows, wrow + 32 * RT) - 1) / G);
-    const int wplain = kParts > 1 ? bplain : uniform(active ? plain_tiles(wrow) : 0);
-    const int wend = kParts > 1 ? ntiles : uniform(active ? (max(0, min(ke, wlast + 1) - kb) + KT - 1) / KT : 0);
-
-    // ---- HBM -> LDS: copy i of a wave fills 16-byte units 64 (w + kWaves i) .. of the tile, lane by lane; the unit's row
-    // and column are those that the swizzle puts there
-    const uint32_t lds0 = lds_addr(smem);
-    const uint8_t *kbase = reinterpret_cast<const uint8_t *>(p.k + (int64_t)(k0 + kb) * p.ks0 + (int64_t)kvh * p.ks1);
-    const uint8_t *vbase = reinterpret_cast<const uint8_t *>(p.v + (int64_t)(k0 + kb) * p.vs0 + (int64_t)kvh * p.vs1);
-    const uint32_t ksb = (uint32_t)(p.ks0 * 2), vsb = (uint32_t)(p.vs0 * 2);
-    auto copy = [&](int t, int stage) {
-      const int left = ke - kb - t * KT - 1;  // the tile's last key (rows past it repeat it: always mapped memory)
-      const uint8_t *kt = kbase + (int64_t)t * KT * ksb, *vt = vbase + (int64_t)t * KT * vsb;
+  // values of keys [key, end) up to row_pos, a lane's channels 32 ct + 0..15 from `row` on, of rows `stride` bytes apart
+  template <int CT>
+  static __device__ __forceinline__ void restore(f32x16_t (&acc)[CT], const uint8_t *row, uint32_t stride, int key, int end,
+                                                 int row_pos) {
+    for (; key < end; ++key, row += stride) {
 #pragma unroll
-      for (int i = 0; i < Sh::kCopies; ++i) {
-        const int at = 64 * (w + Sh::kWaves * i), d = at + lane;
-        const int r = d / U, c = d % U, rs = min(r, left);
-        const uint32_t dst = lds0 + (uint32_t)(stage * Sh::kStage + 16 * at);
-        dma16_saddr<false>(kt, (uint32_t)rs * ksb + 16u * (uint32_t)Sh::k_swz(r, c), dst);
-        dma16_saddr<false>(vt, (uint32_t)rs * vsb + 16u * (uint32_t)Sh::v_swz(r, c), dst + Sh::kHalf);
-      }
-    };
-    // ---- operands. K: row 32 u + col, unit 2 cs + h. V^T: A row 8 q + 4 hh + j of channel tile ct is channel
-    // 32 ct + 16 hh + 4 q + j, so that a lane's accumulators are 16 consecutive channels; the four 4-channel chunks that a
-    // 16-lane group's rows take are then 16 (c & 1) + 4 (c >> 1), and 8 more for the upper group.
-    // A swizzle changes the low bits of a unit's place only: a few lane offsets serve all steps, with the rest immediate.
-    constexpr int kKo = kCs < 8 ? kCs : 8, kVo = kCt < 4 ? kCt : 4;
-    uint32_t koff[kKo], voff[kVo];
+      for (int ct = 0; ct < CT; ++ct) {
+        const u32x4_t y[2] = {*reinterpret_cast<const u32x4_t *>(row + 64 * ct),
+                              *reinterpret_cast<const u32x4_t *>(row + 64 * ct + 16)};
 #pragma unroll
-    for (int i = 0; i < kKo; ++i) koff[i] = col * (2 * HS) + 16 * (Sh::k_swz(col, 2 * i + h) + (kHc / 8) * part);
-    const int vrow = 4 * h + ((lane >> 2) & 3);
-    const int vch = 16 * (lane & 1) + 4 * ((lane >> 1) & 1) + 8 * ((lane >> 4) & 1);
-#pragma unroll
-    for (int i = 0; i < kVo; ++i)
-      voff[i] = vrow * (2 * HS) + 16 * (Sh::v_swz(vrow, 4 * i) + (kHc / 8) * part + (vch >> 3)) + 2 * (vch & 7);
-    auto k_op = [&](const uint8_t *kt, int u, int cs) {
-      return *reinterpret_cast<const u32x4_t *>(kt + koff[cs % kKo] + 32 * u * (2 * HS) + 256 * (cs / kKo));
-    };
-    auto v_op = [&](const uint8_t *vt, int ks, int ct) {
-      u32x4_t r;
-#pragma unroll
-      for (int eight = 0; eight < 2; ++eight) {
-        const uint8_t *at = vt + voff[ct % kVo] + (16 * ks + 8 * eight) * (2 * HS) + 256 * (ct / kVo);
-        const i16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) i16x4_t *)(const __attribute__((address_space(3))) uint8_t *)at);
-        const u32x2_t y = __builtin_bit_cast(u32x2_t, x);
-        r[2 * eight] = y[0];
-        r[2 * eight + 1] = y[1];
-      }
-      return r;
-    };
-
-    auto tile = [&](const uint8_t *kt, int t, auto mask_tag) {
-      constexpr bool MASK = decltype(mask_tag)::value;
-      const uint8_t *vt = kt + Sh::kHalf;
-      f32x16_t s[RT][kSubs];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u) s[rt][u] = f32x16_t{};
-#pragma unroll
-      for (int cs = 0; cs < kCs; ++cs)
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u) {
-          const u32x4_t kop = k_op(kt, u, cs);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) s[rt][u] = mfma_prompt<F16>(kop, qop[rt][cs], s[rt][u]);
-        }
-      if constexpr (kParts > 1) {
-        f32x4_t *own = reinterpret_cast<f32x4_t *>(smem + Sh::kScores + 4096 * w) + lane;
-        const f32x4_t *other = reinterpret_cast<const f32x4_t *>(smem + Sh::kScores + 4096 * (w ^ 1)) + lane;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          own[64 * i] = f32x4_t{s[0][0][4 * i], s[0][0][4 * i + 1], s[0][0][4 * i + 2], s[0][0][4 * i + 3]};
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4_t x = other[64 * i];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[0][0][4 * i + j] += x[j];  // (the same sum in both waves)
+        for (int i = 0; i < 16; ++i) {
+          const uint16_t x = (uint16_t)(y[i >> 3][(i >> 1) & 3] >> (16 * (i & 1)));
+          if ((x & kInf) == kInf && key <= row_pos) acc[ct][i] += from_bits<F16>(x);
         }
       }
-      u32x4_t pop[RT][2 * kSubs];
-      float top[RT];
-      bool raise = false;
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if constexpr (MASK) {
-              const int key = kb + t * KT + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-              if (key > row_pos[rt] || key >= ke) s[rt][u][i] = -INFINITY;
-            }
-            x = fmaxf(x, s[rt][u][i]);
-          }
-        top[rt] = x * p.scale_log2;
-        raise |= top[rt] > m[rt] + kPromptHeadroom;
-      }
-      if (__any(raise)) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const float most = other_half_max(top[rt]);
-          const float to = most > m[rt] + kPromptHeadroom ? most : m[rt];  // (a row's bits do not go by its neighbours)
-          const float alpha = __builtin_amdgcn_exp2f(m[rt] - to);
-          m[rt] = to;
-          l[rt] *= alpha;
-#pragma unroll
-          for (int ct = 0; ct < kCt; ++ct)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[rt][ct][i] *= alpha;
-        }
-      }
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int u = 0; u < kSubs; ++u)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[rt][u][2 * i], p.scale_log2, -m[rt]));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[rt][u][2 * i + 1], p.scale_log2, -m[rt]));
-            l[rt] += p0 + p1;  // (unrounded: the log-sum-exp is kept to fp32)
-            pop[rt][2 * u + (i >> 2)][i & 3] = pack_prompt<F16>(p0, p1);
-          }
-#pragma unroll
-      for (int ks = 0; ks < 2 * kSubs; ++ks)
-#pragma unroll
-        for (int ct = 0; ct < kCt; ++ct) {
-          const u32x4_t vop = v_op(vt, ks, ct);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) acc[rt][ct] = mfma_prompt<F16>(vop, pop[rt][ks], acc[rt][ct]);
-        }
-    };
-
-    // ---- infinities and NaN in V of a tile that some row does not see whole. Such a row's probability is 0, and the MFMA
-    // would make NaN of it: the tile gets zeros in their place (settle), and the rows that see the key the value itself
-    // afterwards, read from memory again (restore): any probability is above 0.
-    constexpr uint32_t kInf = F16 ? 0x7C00u : 0x7F80u;
-    auto odd = [&](uint32_t x) { return ((x & kInf) == kInf) || ((x & (kInf << 16)) == kInf << 16); };
-    auto settle = [&](uint8_t *vt) {
-      uint32_t *vote = reinterpret_cast<uint32_t *>(smem + Sh::kScores);
-      bool any = false;
-      for (int d = tid; d < KT * U; d += Sh::kThreads) {
-        const u32x4_t x = *reinterpret_cast<const u32x4_t *>(vt + 16 * d);
-        any |= odd(x[0]) || odd(x[1]) || odd(x[2]) || odd(x[3]);
-      }
-      if (tid == 0) *vote = 0;
-      __syncthreads();
-      if (any) *vote = 1;
-      __syncthreads();
-      any = *vote != 0;
-      if constexpr (kParts > 1) __syncthreads();  // (the word lies where the next scores go)
-      if (!any) return false;
-      for (int d = tid; d < KT * U; d += Sh::kThreads) {
-        u32x4_t x = *reinterpret_cast<const u32x4_t *>(vt + 16 * d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if ((x[j] & kInf) == kInf) x[j] &= 0xFFFF0000u;
-          if ((x[j] & (kInf << 16)) == kInf << 16) x[j] &= 0xFFFFu;
-        }
-        *reinterpret_cast<u32x4_t *>(vt + 16 * d) = x;
-      }
-      __syncthreads();
-      return true;
-    };
-    auto restore = [&](int t) {
-      for (int key = kb + t * KT; key < min(ke, kb + (t + 1) * KT); ++key) {
-        const uint8_t *row = vbase + (int64_t)(key - kb) * vsb + 2 * (kHc * part + 16 * h);
-#pragma unroll
-        for (int ct = 0; ct < kCt; ++ct) {
-          const u32x4_t y[2] = {*reinterpret_cast<const u32x4_t *>(row + 64 * ct),
-                                *reinterpret_cast<const u32x4_t *>(row + 64 * ct + 16)};
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint16_t x = (uint16_t)(y[i >> 3][(i >> 1) & 3] >> (16 * (i & 1)));
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              if ((x & kInf) == kInf && key <= row_pos[rt]) acc[rt][ct][i] += from_bits<F16>(x);
-          }
-        }
-      }
-    };
-
-    // ---- the walk: kStages - 1 tiles in flight; each iteration waits for its own, and the barrier after that also says
-    // that every wave has left the stage which the next copy fills
-    constexpr int kAhead = Sh::kStages - 1;
-#pragma unroll
-    for (int t = 0; t < kAhead; ++t)
-      if (t < ntiles) copy(t, t);
-    int stage = 0;
-    for (int t = 0; t < ntiles; ++t) {
-      if (kAhead == 1 || t + 1 >= ntiles) wait_vmcnt<0>();
-      else wait_vmcnt<2 * Sh::kCopies>();
-      __syncthreads();
-      const int into = stage == 0 ? Sh::kStages - 1 : stage - 1;
-      if (t + kAhead < ntiles) copy(t + kAhead, into);
-      uint8_t *kt = smem + stage * Sh::kStage;
-      const bool odd_values = t >= bplain && settle(kt + Sh::kHalf);
-      if (t < wplain) tile(kt, t, std::false_type{});
-      else if (t < wend) tile(kt, t, std::true_type{});
-      if (odd_values && active) restore(t);
-      stage = stage + 1 == Sh::kStages ? 0 : stage + 1;
     }
   }
+};
 
-  // ---- epilogue: a lane's 16 consecutive channels of each channel tile
+// Whether 32 rows of a V tile hold any, for the whole wave.
+template <int HS, bool F16>
+__device__ __forceinline__ bool odd_values(const uint8_t *vt, int lane) {
+  u16x2_t most = {0, 0};
+#pragma unroll 2
+  for (int d = lane; d < 32 * HS / 8; d += 64) {
+    const u32x4_t x = *reinterpret_cast<const u32x4_t *>(vt + 16 * d);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const float sum = l[rt] + shfl_xor_f(l[rt], 32);
-    if (tok[rt] < 0) continue;
-    const int64_t t = q0 + tok[rt], head = kvh * G + jh[rt];
-    if (S == 1) {
-      const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (a sum that is no number stays none)
-      uint16_t *orow = p.out + t * p.os0 + head * p.os1 + kHc * part + 16 * h;
+    for (int j = 0; j < 4; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, x[j] & 0x7FFF7FFFu));
+  }
+  return __any(most[0] >= Odd<F16>::kInf || most[1] >= Odd<F16>::kInf);
+}
+
+// The largest of a lane's 16 scores.
+__device__ __forceinline__ float largest(const f32x16_t &x) {
+  float a = fmaxf(fmaxf(x[0], x[1]), x[2]), b = fmaxf(fmaxf(x[3], x[4]), x[5]);
+  a = fmaxf(fmaxf(a, x[6]), x[7]);
+  b = fmaxf(fmaxf(b, x[8]), x[9]);
+  a = fmaxf(fmaxf(a, x[10]), x[11]);
+  b = fmaxf(fmaxf(b, x[12]), x[13]);
+  a = fmaxf(fmaxf(a, x[14]), x[15]);
+  return fmaxf(a, b);
+}
+
+// Scores of keys past the row's position or the split's end are -inf; key0: the key of the lane's first score.
+__device__ __forceinline__ void mask_scores(f32x16_t &x, int key0, int row_pos, int ke) {
 #pragma unroll
-      for (int ct = 0; ct < kCt; ++ct)
+  for (int i = 0; i < 16; ++i) {
+    const int key = key0 + 8 * (i >> 2) + (i & 3);
+    if (key > row_pos || key >= ke) x[i] = -INFINITY;
+  }
+}
+
+// A row's maximum m is raised to `top` (the largest score of the lane's keys) where that exceeds it by the headroom, and
+// what was summed up relative to the old one is scaled. A row's bits do not go by its neighbours': each is raised for itself.
+template <int CT>
+__device__ __forceinline__ void raise(float top, float scale_log2, float &m, float &l, f32x16_t (&acc)[CT]) {
+  top *= scale_log2;
+  if (__any(top > m + kPromptHeadroom)) {
+    const float most = other_half_max(top);
+    const float to = most > m + kPromptHeadroom ? most : m;
+    const float alpha = __builtin_amdgcn_exp2f(m - to);
+    m = to;
+    l *= alpha;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          u32x4_t y;
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            y[j] = pack_prompt<F16>(acc[rt][ct][8 * i + 2 * j] * inv, acc[rt][ct][8 * i + 2 * j + 1] * inv);
-          *reinterpret_cast<u32x4_t *>(orow + 32 * ct + 8 * i) = y;
-        }
-      if (p.lse && h == 0 && part == 0)
-        p.lse[t * p.ls0 + head * p.ls1] = sum != 0.f ? (m[rt] + log2f(sum)) * (1.f / kLog2e) : -INFINITY;
-    } else {
-      const int64_t at = (t * p.num_q_heads + head) * S + split;
-      float *orow = p.so + at * HS + kHc * part + 16 * h;
+      for (int i = 0; i < 16; ++i) acc[ct][i] *= alpha;
+  }
+}
+
+// A row's result: channels 32 ct + 16 h + 0..15 of `channel` on, to out or to the split's partial.
+template <int HS, bool F16, int CT>
+__device__ __forceinline__ void store_row(const PromptParams &p, const PromptBlock &b, int tok, int jh, int channel, bool stats,
+                                          float m, float sum, const f32x16_t (&acc)[CT]) {
+  if (tok < 0) return;
+  const int64_t t = b.q0 + tok, head = b.kvh * (p.num_q_heads / p.num_kv_heads) + jh;
+  if (p.num_splits == 1) {
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;  // (a sum that is no number stays none)
+    uint16_t *orow = p.out + t * p.os0 + head * p.os1 + channel;
 #pragma unroll
-      for (int ct = 0; ct < kCt; ++ct)
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<float4 *>(orow + 32 * ct + i) =
-              make_float4(acc[rt][ct][i], acc[rt][ct][i + 1], acc[rt][ct][i + 2], acc[rt][ct][i + 3]);
-      if (h == 0 && part == 0) {
-        p.smax[at] = m[rt];
-        p.ssum[at] = sum;
+      for (int i = 0; i < 2; ++i) {
+        u32x4_t y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = pack_prompt<F16>(acc[ct][8 * i + 2 * j] * inv, acc[ct][8 * i + 2 * j + 1] * inv);
+        *reinterpret_cast<u32x4_t *>(orow + 32 * ct + 8 * i) = y;
       }
+    if (p.lse && stats)
+      p.lse[t * p.ls0 + head * p.ls1] = sum != 0.f ? (m + log2f(sum)) * (1.f / kLog2e) : -INFINITY;
+  } else {
+    const int64_t at = (t * p.num_q_heads + head) * p.num_splits + b.split;
+    float *orow = p.so + at * HS + channel;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4 *>(orow + 32 * ct + i) = make_float4(acc[ct][i], acc[ct][i + 1], acc[ct][i + 2], acc[ct][i + 3]);
+    if (stats) {
+      p.smax[at] = m;
+      p.ssum[at] = sum;
     }
   }
 }
 
-// The log-sum-exp merge of split partials, a wave per (token, query head) row: the row's splits weighed by 2^(m - max m).
-template <int HS, bool F16>
-__global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptParams p) {
-  constexpr int E = HS / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t t = row / p.num_q_heads, head = row - t * p.num_q_heads;
-  if (t >= p.num_tokens) return;
-  int lo = 0, hi = p.num_seqs - 1;  // the last sequence that starts at or before the token
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu_q[mid] <= t) lo = mid;
-    else hi = mid - 1;
+// ------------------------------------------------------------------------------------- heads of 64, 128 and 256
+
+template <int HS_, bool F16_>
+struct PromptShape {
+  static constexpr int HS = HS_;
+  static constexpr bool F16 = F16_;
+  // Two waves per SIMD up to head 128, in one workgroup at 128, whose tiles then serve 256 rows, and in two at 64 (60 us
+  // against 63 on four sequences of up to 509 tokens over up to 4605 keys). At 256 a wave takes 512 registers.
+  static constexpr int kWaves = HS == 128 ? 8 : 4;
+  static constexpr int kWavesPerSimd = HS <= 128 ? 2 : 1;
+  static constexpr int kThreads = kWaves * 64;
+  static constexpr int kRows = kWaves * 32;
+  static constexpr int kKeys = 64;                   // keys per tile, two sub-tiles of 32
+  static constexpr int kU = HS / 8;                  // 16-byte units of a row
+  static constexpr int kTile = kKeys * HS * 2;       // bytes of a tile's K (and of its V)
+  static constexpr int kKRing = 2, kVRing = 3;       // tiles of K and V in LDS
+  static constexpr int kOffV = kKRing * kTile;
+  static constexpr int kLds = kOffV + kVRing * kTile;
+  static constexpr int kCopies = kTile / 1024 / kWaves;  // 1 KiB copies of a wave, K and V each
+  static_assert(kTile % (1024 * kWaves) == 0 && kLds <= 160 * 1024, "LDS");
+  // Position of unit c in row r of a K tile: 16 rows' reads of one unit hit every bank of the LDS once.
+  static __host__ __device__ constexpr int k_swz(int r, int c) { return HS == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15); }
+  // The same in a V tile, in blocks of four units (32 channels, what a transposing read takes of a row): the four rows of
+  // a 16-lane group hit different banks. At head 64 a row has two blocks, and two rows every bank.
+  static __host__ __device__ constexpr int v_swz(int r, int c) {
+    return HS == 64 ? c ^ (((r >> 1) & 1) << 2) : c ^ ((r & 3) << 2);
   }
-  if (t < p.cu_q[lo] || t >= p.cu_q[lo + 1]) return;  // a row of no sequence: left as it is
-  const int k0 = max(0, p.cu_k[lo]), n = max(0, min(p.cu_k[lo + 1], p.num_keys) - k0);
+};
+
+template <class Sh>
+__global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel(const PromptParams p) {
+  constexpr int HS = Sh::HS, KT = Sh::kKeys, U = Sh::kU;
+  constexpr bool F16 = Sh::F16;
+  constexpr int kCs = HS / 16, kCt = HS / 32;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[Sh::kLds];
+  PromptBlock b;
+  if (!prompt_block<Sh::kRows>(p, b)) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const int G = p.num_q_heads / p.num_kv_heads;
+  const int kb = b.kb, ke = b.ke;
+  auto last_pos = [&](int row) { return p.causal ? b.n - b.qlen + row / G : b.n - 1; };  // the last key that a row sees
+
+  // ---- the wave's rows: lane row col -> (token rr / G, query head rr % G)
+  const int wrow = b.r0 + 32 * w, rr = wrow + col;
+  const bool active = wrow < b.nrows, valid = rr < b.nrows;
+  const int tok = valid ? rr / G : -1, jh = valid ? rr - tok * G : 0;
+  const int row_pos = valid ? last_pos(rr) : -1;
+  u32x4_t qop[kCs];
+  {
+    const uint16_t *src = p.q + (int64_t)(b.q0 + max(0, tok)) * p.qs0 + (int64_t)(b.kvh * G + jh) * p.qs1 + 8 * h;
+#pragma unroll
+    for (int cs = 0; cs < kCs; ++cs)
+      qop[cs] = valid ? *reinterpret_cast<const u32x4_t *>(src + 16 * cs) : u32x4_t{0u, 0u, 0u, 0u};
+  }
+  f32x16_t acc[kCt];
+  float m = kPromptNone, l = 0.f;
+#pragma unroll
+  for (int ct = 0; ct < kCt; ++ct) acc[ct] = f32x16_t{};
+
+  const int ntiles = ke > kb ? (ke - kb + KT - 1) / KT : 0;
+  if (ntiles > 0) {
+    auto seen = [&](int row) { return max(0, min(last_pos(row) + 1, ke) - kb); };  // keys of the split that a row sees
+    const int wplain = uniform(active ? seen(wrow) : 0) / 32;  // sub-tiles that every row of the wave sees whole,
+    const int wend = uniform(active ? seen(min(b.nrows, wrow + 32) - 1) + 31 : 0) / 32;  // and that some row sees at all
+
+    // ---- HBM -> LDS: copy i of a wave fills 16-byte units 64 (w + kWaves i) .. of the tile, lane by lane; the unit's row
+    // and column are those that the swizzle puts there
+    const uint32_t lds0 = lds_addr(smem);
+    const uint8_t *kbase = reinterpret_cast<const uint8_t *>(p.k + (int64_t)(b.k0 + kb) * p.ks0 + (int64_t)b.kvh * p.ks1);
+    const uint8_t *vbase = reinterpret_cast<const uint8_t *>(p.v + (int64_t)(b.k0 + kb) * p.vs0 + (int64_t)b.kvh * p.vs1);
+    const uint32_t ksb = (uint32_t)(p.ks0 * 2), vsb = (uint32_t)(p.vs0 * 2);
+    uint32_t kvo[Sh::kCopies], vvo[Sh::kCopies];  // the lane's byte offsets in a whole tile
+#pragma unroll
+    for (int i = 0; i < Sh::kCopies; ++i) {
+      const int d = 64 * (w + Sh::kWaves * i) + lane, r = d / U, c = d % U;
+      kvo[i] = (uint32_t)r * ksb + 16u * (uint32_t)Sh::k_swz(r, c);
+      vvo[i] = (uint32_t)r * vsb + 16u * (uint32_t)Sh::v_swz(r, c);
+    }
+    auto copy = [&](int t, int kslot, int vslot) {
+      const int left = ke - kb - t * KT - 1;  // the tile's last key (rows past it repeat it: always mapped memory)
+      const uint8_t *kt = kbase + (int64_t)t * KT * ksb, *vt = vbase + (int64_t)t * KT * vsb;
+#pragma unroll
+      for (int i = 0; i < Sh::kCopies; ++i) {
+        const int at = 64 * (w + Sh::kWaves * i);
+        uint32_t ko = kvo[i], vo = vvo[i];
+        if (left < KT - 1) {
+          const int d = at + lane, r = d / U, c = d % U, rs = min(r, left);
+          ko = (uint32_t)rs * ksb + 16u * (uint32_t)Sh::k_swz(r, c);
+          vo = (uint32_t)rs * vsb + 16u * (uint32_t)Sh::v_swz(r, c);
+        }
+        dma16_saddr<false>(kt, ko, lds0 + (uint32_t)(kslot * Sh::kTile + 16 * at));
+        dma16_saddr<false>(vt, vo, lds0 + (uint32_t)(Sh::kOffV + vslot * Sh::kTile + 16 * at));
+      }
+    };
+    // ---- operands. A swizzle changes the low bits of a unit's place only: a few lane offsets serve all steps, with the rest
+    // immediate.
+    constexpr int kKo = kCs < 8 ? kCs : 8, kVo = kCt < 4 ? kCt : 4;
+    uint32_t koff[kKo], voff[kVo];
+#pragma unroll
+    for (int i = 0; i < kKo; ++i) koff[i] = col * (2 * HS) + 16 * Sh::k_swz(col, 2 * i + h);
+#pragma unroll
+    for (int i = 0; i < kVo; ++i)
+      voff[i] = v_row(lane) * (2 * HS) + 16 * Sh::v_swz(v_row(lane), 4 * i) + 2 * v_channel(lane);
+    auto k_op = [&](const uint8_t *kt, int cs) {
+      return *reinterpret_cast<const u32x4_t *>(kt + koff[cs % kKo] + 256 * (cs / kKo));
+    };
+    auto v_op = [&](const uint8_t *vt, int ks, int ct) {
+      return v_operand<HS>(vt + voff[ct % kVo] + 32 * ks * HS + 256 * (ct / kVo));
+    };
+
+    f32x16_t s;  // the running sub-tile's scores
+    // Sub-tile g's softmax and second product beside the scores of g + 1. MASK: some row may not see all of g + 1 (or none
+    // of it: whatever lies in its place is then masked). ODD: sub-tile g's values hold infinities or NaN.
+    auto body = [&](const uint8_t *kn, const uint8_t *vt, int g, auto mask_tag, auto odd_tag) {
+      constexpr bool MASK = decltype(mask_tag)::value, ODD = decltype(odd_tag)::value;
+      constexpr int kP = 2 * kCt, kPre = 2;
+      f32x16_t sn = {}, sn2 = {};
+      u32x4_t kbuf[kPre], vbuf[kPre], pop[2];
+#pragma unroll
+      for (int c = 0; c < kPre; ++c) {
+        kbuf[c] = k_op(kn, c);
+        vbuf[c] = v_op(vt, c / kCt, c % kCt);
+      }
+      auto pair = [&](int i) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * i], p.scale_log2, -m));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], p.scale_log2, -m));
+        l += p0 + p1;  // (unrounded: the log-sum-exp is kept to fp32)
+        pop[i >> 2][i & 3] = pack_prompt<F16>(p0, p1);
+      };
+      constexpr int kFirst = 6;    // pairs beside the first product, the others beside the second
+      constexpr bool kTwo = HS == 256;  // two chains of MFMAs for the scores where one wave has a SIMD for itself
+#pragma unroll
+      for (int c = 0; c < kCs; ++c) {
+        const u32x4_t kop = kbuf[c % kPre];
+        if (c + kPre < kCs) kbuf[c % kPre] = k_op(kn, c + kPre);
+        if (kTwo && (c & 1)) sn2 = mfma_prompt<F16>(kop, qop[c], sn2);
+        else sn = mfma_prompt<F16>(kop, qop[c], sn);
+#pragma unroll
+        for (int i = 0; i < kFirst; ++i)
+          if (i * kCs / kFirst == c) pair(i);
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < kP; ++c) {
+        u32x4_t vop = vbuf[c % kPre];
+        if constexpr (ODD) vop = Odd<F16>::without(vop);
+        if (c + kPre < kP) vbuf[c % kPre] = v_op(vt, (c + kPre) / kCt, (c + kPre) % kCt);
+        acc[c % kCt] = mfma_prompt<F16>(vop, pop[c / kCt], acc[c % kCt]);
+        if (c < kCt) {
+#pragma unroll
+          for (int i = kFirst; i < 8; ++i)
+            if ((i - kFirst) * kCt / (8 - kFirst) == c) pair(i);
+        }
+        if (c == kP / 2) {
+          if constexpr (kTwo) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sn[i] += sn2[i];
+          }
+          if constexpr (MASK) mask_scores(sn, kb + 32 * (g + 1) + 4 * h, row_pos, ke);
+          top = largest(sn);
+        }
+      }
+      s = sn;
+      raise(top, p.scale_log2, m, l, acc);
+    };
+
+    // ---- the walk. Tile t's last sub-tile is worked through beside the first scores of tile t + 1: before it the waves
+    // meet, tile t + 1 having landed. Then every wave is past tile t's scores and tile t - 1's values, and tile t + 2 is
+    // copied in their place.
+    using No = std::false_type;
+    using Yes = std::true_type;
+    copy(0, 0, 0);
+    if (ntiles > 1) {
+      copy(1, 1, 1);
+      wait_vmcnt<2 * Sh::kCopies>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    __syncthreads();
+    if (wend > 0) {
+      s = f32x16_t{};
+#pragma unroll
+      for (int c = 0; c < kCs; ++c) s = mfma_prompt<F16>(k_op(smem, c), qop[c], s);
+      if (wplain == 0) mask_scores(s, kb + 4 * h, row_pos, ke);
+      raise(largest(s), p.scale_log2, m, l, acc);
+    }
+    int t = 0, vslot = 0;
+    auto k_at = [&](int t) { return smem + (t & 1) * Sh::kTile; };
+    auto meet = [&] {
+      wait_vmcnt<0>();
+      __syncthreads();
+      if (t + 2 < ntiles) copy(t + 2, t & 1, vslot == 0 ? 2 : vslot - 1);
+    };
+    for (; 2 * t + 2 < wplain; ++t) {  // both sub-tiles, and the one after, are seen whole by every row
+      const uint8_t *vt = smem + Sh::kOffV + vslot * Sh::kTile;
+      body(k_at(t) + 64 * HS, vt, 2 * t, No{}, No{});
+      meet();
+      body(k_at(t + 1), vt + 64 * HS, 2 * t + 1, No{}, No{});
+      vslot = vslot == 2 ? 0 : vslot + 1;
+    }
+    for (; t < ntiles; ++t) {
+      const uint8_t *tile = smem + Sh::kOffV + vslot * Sh::kTile;
+#pragma unroll 1
+      for (int u = 0; u < 2; ++u) {
+        if (u == 1) meet();
+        const int g = 2 * t + u;
+        if (g >= wend) continue;
+        const uint8_t *kn = u == 0 ? k_at(t) + 64 * HS : k_at(t + 1), *vt = tile + u * 64 * HS;
+        if (g >= wplain && odd_values<HS, F16>(vt, lane)) {
+          body(kn, vt, g, Yes{}, Yes{});
+          Odd<F16>::restore(acc, vbase + (int64_t)(32 * g) * vsb + 32 * h, vsb, kb + 32 * g, min(ke, kb + 32 * g + 32), row_pos);
+        } else {
+          body(kn, vt, g, Yes{}, No{});
+        }
+      }
+      vslot = vslot == 2 ? 0 : vslot + 1;
+    }
+  }
+  store_row<HS, F16>(p, b, tok, jh, 16 * h, h == 0, m, l + shfl_xor_f(l, 32), acc);
+}
+
+// -------------------------------------------------------------------------------------------- heads of 512
+//
+// A row tile's accumulators and query operands would take 384 registers: two waves share it, each with half of the channels
+// of q, K, V and out. Each makes the scores of its channels, and the two parts are added through LDS; both then have the same
+// bits and make the same probabilities.
+
+template <bool F16>
+__global__ __launch_bounds__(256) void prompt_wide_kernel(const PromptParams p) {
+  constexpr int HS = 512, KT = 32, U = HS / 8, kHc = HS / 2, kWaves = 4;
+  constexpr int kCs = kHc / 16, kCt = kHc / 32;
+  constexpr int kTile = KT * HS * 2, kStage = 2 * kTile, kScores = 2 * kStage, kCopies = kTile / 1024 / kWaves;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kScores + kWaves * 4096];
+  auto k_swz = [](int r, int c) { return c ^ (r & 15); };
+  auto v_swz = [](int r, int c) { return c ^ ((r & 3) << 2); };
+  PromptBlock b;
+  if (!prompt_block<kPromptWideRows>(p, b)) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+  const int col = lane & 31, h = lane >> 5, part = w & 1;
+  const int G = p.num_q_heads / p.num_kv_heads;
+  const int kb = b.kb, ke = b.ke;
+  auto last_pos = [&](int row) { return p.causal ? b.n - b.qlen + row / G : b.n - 1; };
+  const int rr = b.r0 + 32 * (w >> 1) + col;
+  const bool valid = rr < b.nrows;
+  const int tok = valid ? rr / G : -1, jh = valid ? rr - tok * G : 0;
+  const int row_pos = valid ? last_pos(rr) : -1;
+  u32x4_t qop[kCs];
+  const uint16_t *src = p.q + (int64_t)(b.q0 + max(0, tok)) * p.qs0 + (int64_t)(b.kvh * G + jh) * p.qs1 + kHc * part + 8 * h;
+#pragma unroll
+  for (int cs = 0; cs < kCs; ++cs)
+    qop[cs] = valid ? *reinterpret_cast<const u32x4_t *>(src + 16 * cs) : u32x4_t{0u, 0u, 0u, 0u};
+  f32x16_t acc[kCt];
+  float m = kPromptNone, l = 0.f;
+#pragma unroll
+  for (int ct = 0; ct < kCt; ++ct) acc[ct] = f32x16_t{};
+
+  const int ntiles = ke > kb ? (ke - kb + KT - 1) / KT : 0;
+  if (ntiles > 0) {
+    const int plain = uniform(max(0, min(last_pos(b.r0) + 1, ke) - kb) / KT);  // tiles that every row of the block sees whole
+    const uint32_t lds0 = lds_addr(smem);
+    const uint8_t *kbase = reinterpret_cast<const uint8_t *>(p.k + (int64_t)(b.k0 + kb) * p.ks0 + (int64_t)b.kvh * p.ks1);
+    const uint8_t *vbase = reinterpret_cast<const uint8_t *>(p.v + (int64_t)(b.k0 + kb) * p.vs0 + (int64_t)b.kvh * p.vs1);
+    const uint32_t ksb = (uint32_t)(p.ks0 * 2), vsb = (uint32_t)(p.vs0 * 2);
+    auto copy = [&](int t) {  // a copy is one row: 64 units
+      const int left = ke - kb - t * KT - 1;
+      const uint8_t *kt = kbase + (int64_t)t * KT * ksb, *vt = vbase + (int64_t)t * KT * vsb;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int r = w + kWaves * i, rs = min(r, left);
+        const uint32_t dst = lds0 + (uint32_t)((t & 1) * kStage + 1024 * r);
+        dma16_saddr<false>(kt + (int64_t)rs * ksb, 16u * (uint32_t)k_swz(r, lane), dst);
+        dma16_saddr<false>(vt + (int64_t)rs * vsb, 16u * (uint32_t)v_swz(r, lane), dst + kTile);
+      }
+    };
+    uint32_t koff[8], voff[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) koff[i] = col * (2 * HS) + 16 * (k_swz(col, 2 * i + h) + (kHc / 8) * part);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      voff[i] = v_row(lane) * (2 * HS) + 16 * (v_swz(v_row(lane), 4 * i) + (kHc / 8) * part) + 2 * v_channel(lane);
+    auto tile = [&](const uint8_t *kt, int t, auto mask_tag) {
+      constexpr bool MASK = decltype(mask_tag)::value;
+      const uint8_t *vt = kt + kTile;
+      auto v_op = [&](int c) { return v_operand<HS>(vt + voff[c % kCt % 4] + 32 * (c / kCt) * HS + 256 * (c % kCt / 4)); };
+      f32x16_t s = {}, s2 = {};
+#pragma unroll
+      for (int cs = 0; cs < kCs; ++cs) {
+        const u32x4_t kop = *reinterpret_cast<const u32x4_t *>(kt + koff[cs % 8] + 256 * (cs / 8));
+        if (cs & 1) s2 = mfma_prompt<F16>(kop, qop[cs], s2);
+        else s = mfma_prompt<F16>(kop, qop[cs], s);
+      }
+      f32x4_t *own = reinterpret_cast<f32x4_t *>(smem + kScores + 4096 * w) + lane;
+      const f32x4_t *other = reinterpret_cast<const f32x4_t *>(smem + kScores + 4096 * (w ^ 1)) + lane;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] += s2[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) own[64 * i] = f32x4_t{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4_t x = other[64 * i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[4 * i + j] += x[j];
+      }
+      if constexpr (MASK) mask_scores(s, kb + t * KT + 4 * h, row_pos, ke);
+      raise(largest(s), p.scale_log2, m, l, acc);
+      u32x4_t pop[2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * i], p.scale_log2, -m));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], p.scale_log2, -m));
+        l += p0 + p1;
+        pop[i >> 2][i & 3] = pack_prompt<F16>(p0, p1);
+      }
+#pragma unroll
+      for (int c = 0; c < 2 * kCt; ++c) acc[c % kCt] = mfma_prompt<F16>(v_op(c), pop[c / kCt], acc[c % kCt]);
+    };
+    // zeros in the place of a tile's infinities and NaN; whether there were any
+    auto settle = [&](uint8_t *vt) {
+      const bool odd = odd_values<HS, F16>(vt, lane);  // (every wave looks at all of it)
+      __syncthreads();
+      if (!odd) return false;
+      for (int d = tid; d < KT * U; d += 256)
+        *reinterpret_cast<u32x4_t *>(vt + 16 * d) = Odd<F16>::without(*reinterpret_cast<u32x4_t *>(vt + 16 * d));
+      __syncthreads();
+      return true;
+    };
+    // one tile in flight; the barrier says that it has landed, and that every wave has left the other stage
+    copy(0);
+    for (int t = 0; t < ntiles; ++t) {
+      wait_vmcnt<0>();
+      __syncthreads();
+      if (t + 1 < ntiles) copy(t + 1);
+      uint8_t *kt = smem + (t & 1) * kStage;
+      if (t < plain) {
+        tile(kt, t, std::false_type{});
+        continue;
+      }
+      const bool odd = settle(kt + kTile);
+      tile(kt, t, std::true_type{});
+      if (odd)
+        Odd<F16>::restore(acc, vbase + (int64_t)t * KT * vsb + 2 * (kHc * part + 16 * h), vsb, kb + t * KT,
+                          min(ke, kb + (t + 1) * KT), row_pos);
+    }
+  }
+  store_row<HS, F16>(p, b, tok, jh, kHc * part + 16 * h, h == 0 && part == 0, m, l + shfl_xor_f(l, 32), acc);
+}
+
+// The log-sum-exp merge of split partials, kPer waves per (token, query head) row: the row's splits weighed by
+// 2^(m - max m). A wave has its splits' statistics in its lanes and takes 8 splits' channels at a time, all loads issued
+// before any is used.
+template <int HS, bool F16, int kPer>
+__global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptParams p) {
+  constexpr int E = HS / 64, kBatch = 8;
+  __shared__ float part[kPer > 1 ? (kPer - 1) * HS : 1];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wr = w % kPer;
+  const int64_t row = (int64_t)blockIdx.x * (4 / kPer) + w / kPer;
+  const int t = (int)(row / p.num_q_heads), head = (int)(row - (int64_t)t * p.num_q_heads);
+  if (t >= p.num_tokens) return;  // (with kPer 4 a workgroup has one row: all of it returns)
+  int seq = -1, k0 = 0, k1 = 0;   // the last sequence that starts at or before the token
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 63) {
+    const int i = min(s0 + lane, p.num_seqs);
+    const int cq = p.cu_q[i], ck = p.cu_k[i];
+    const uint64_t before = __ballot(s0 + lane < p.num_seqs && lane < 63 && cq <= t);
+    if (!before) break;
+    const int at = 63 - __builtin_clzll(before);
+    seq = t < __builtin_amdgcn_readlane(cq, at + 1) ? s0 + at : -1;
+    k0 = __builtin_amdgcn_readlane(ck, at);
+    k1 = __builtin_amdgcn_readlane(ck, at + 1);
+    if (at < 62) break;
+  }
+  if (seq < 0) return;  // a row of no sequence: left as it is
+  k0 = max(0, k0);
+  const int n = max(0, min(k1, p.num_keys) - k0);
   const int seg = segment_keys(n, p.num_splits, p.min_keys);
   const int used = min(p.num_splits, (int)(((int64_t)n + seg - 1) / seg));
   const float *smax = p.smax + row * p.num_splits, *ssum = p.ssum + row * p.num_splits;
-  const float *so = p.so + row * p.num_splits * HS + E * lane;
-  float top = kPromptNone;
-  for (int s = 0; s < used; ++s) top = fmaxf(top, smax[s]);
-  float sum = 0.f, x[E] = {};
-  for (int s = 0; s < used; ++s) {
-    const float f = __builtin_amdgcn_exp2f(smax[s] - top);
-    sum = fmaf(ssum[s], f, sum);
+  const float m0 = lane < used ? smax[lane] : kPromptNone, m1 = lane + 64 < used ? smax[lane + 64] : kPromptNone;
+  const float l0 = lane < used ? ssum[lane] : 0.f, l1 = lane + 64 < used ? ssum[lane + 64] : 0.f;
+  float top = fmaxf(m0, m1);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = fmaf(so[(int64_t)s * HS + e], f, x[e]);
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, shfl_xor_f(top, o));
+  const float f0 = __builtin_amdgcn_exp2f(m0 - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+  float sum = fmaf(l0, f0, l1 * f1);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) sum += shfl_xor_f(sum, o);
+  const float *so = p.so + row * p.num_splits * HS + E * lane;
+  float x[E] = {};
+  for (int s0 = wr * kBatch; s0 < used; s0 += kPer * kBatch) {
+    float v[kBatch][E];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int s = min(s0 + i, used - 1);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i][e] = so[(int64_t)s * HS + e];
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int s = s0 + i;
+      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s < 64 ? f0 : f1), s & 63));
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (s < used) x[e] = fmaf(v[i][e], f, x[e]);
+    }
+  }
+  if constexpr (kPer > 1) {
+    if (wr > 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) part[(wr - 1) * HS + E * lane + e] = x[e];
+    }
+    __syncthreads();
+    if (wr > 0) return;
+#pragma unroll
+    for (int i = 0; i < kPer - 1; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] += part[i * HS + E * lane + e];
   }
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   uint16_t *orow = p.out + t * p.os0 + head * p.os1 + E * lane;
@@ -463,7 +709,7 @@ template <int HS>
 constexpr int prompt_rows() { return PromptShape<HS, false>::kRows; }
 
 int prompt_block_rows(int hs) {
-  return hs == 64 ? prompt_rows<64>() : hs == 128 ? prompt_rows<128>() : hs == 256 ? prompt_rows<256>() : prompt_rows<512>();
+  return hs == 64 ? prompt_rows<64>() : hs == 128 ? prompt_rows<128>() : hs == 256 ? prompt_rows<256>() : kPromptWideRows;
 }
 
 // Workgroups of one key split at most: sequence s owns row blocks [cu_q[s] G / R + s, cu_q[s + 1] G / R + s + 1) of R rows.
@@ -476,12 +722,19 @@ constexpr int kPromptSplitKeys = 256;
 
 int prompt_splits(const qp_prompt_args *a) {
   if (a->num_splits > 0) return a->num_splits;
-  const int64_t wgs = prompt_blocks(a) * a->num_kv_heads, cus = device_cus();
+  const int64_t cus = device_cus(), G = a->num_q_heads / a->num_kv_heads, rows = prompt_block_rows(a->head_size);
+  const int64_t filled = ((int64_t)a->num_tokens * G + rows - 1) / rows;  // (every sequence has a block of its own, too)
+  const int64_t wgs = (filled > a->num_seqs ? filled : a->num_seqs) * a->num_kv_heads;
   if (wgs >= cus) return 1;
-  int64_t s = (2 * cus + wgs - 1) / wgs;
-  const int64_t most = a->max_seqlen_k / kPromptSplitKeys;
-  if (s > most) s = most;
-  return s < 1 ? 1 : s > 128 ? 128 : (int)s;
+  const double tiles = a->max_seqlen_k / 64.0, out = (double)a->num_tokens * a->num_q_heads * a->head_size;
+  auto cost = [&](int64_t s) {
+    return (double)((wgs * s + cus - 1) / cus) * (tiles / s + 6) + (s > 1 ? 6 + out * s * 2e-6 : 0);
+  };
+  int64_t most = a->max_seqlen_k / kPromptSplitKeys, best = 1;
+  if (most > 128) most = 128;
+  for (int64_t s = 2; s <= most; ++s)
+    if (cost(s) < cost(best)) best = s;
+  return (int)best;
 }
 
 int64_t prompt_partial_bytes(const qp_prompt_args *a, int splits) {
@@ -491,11 +744,14 @@ int64_t prompt_partial_bytes(const qp_prompt_args *a, int splits) {
 
 template <int HS, bool F16>
 void launch_prompt(const PromptParams &p, dim3 grid, hipStream_t s) {
-  using Sh = PromptShape<HS, F16>;
-  prompt_kernel<Sh><<<grid, Sh::kThreads, 0, s>>>(p);
+  const uint32_t share = prompt_share(grid.y * grid.z);
+  grid.x = ((grid.x + (1u << share) - 1) >> share) << share;
+  if constexpr (HS == 512) prompt_wide_kernel<F16><<<grid, 256, 0, s>>>(p);
+  else prompt_kernel<PromptShape<HS, F16>><<<grid, PromptShape<HS, F16>::kThreads, 0, s>>>(p);
   if (p.num_splits > 1) {
     const int64_t rows = (int64_t)p.num_tokens * p.num_q_heads;
-    prompt_merge_kernel<HS, F16><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(p);
+    if (p.num_splits > 8) prompt_merge_kernel<HS, F16, 4><<<(unsigned)rows, 256, 0, s>>>(p);
+    else prompt_merge_kernel<HS, F16, 1><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(p);
   }
 }
 
