@@ -44,6 +44,7 @@ struct KeyWeightParams {
 constexpr int kKwWaves = 4;
 constexpr int kKwThreads = kKwWaves * 64;
 constexpr int kKwSubs = 4;              // 32-key tiles of a wave at most
+constexpr int kKwBlocks = 8;           // blocks of keys of a workgroup at most (many rows)
 constexpr float kKwNone = -1e30f;       // the maximum of a row that has seen no key
 
 typedef uint32_t u32x4_words_t __attribute__((ext_vector_type(4), aligned(4)));
@@ -118,20 +119,22 @@ __device__ __forceinline__ u32x4_t load_row(const KeyWeightParams &p, int q0, in
   return v;
 }
 
-// A key's page (-1: past the context, or not a page of the cache).
-__device__ __forceinline__ int key_page(const KeyWeightParams &p, const int32_t *trow, int key, int n, int &slot) {
+// A key's entry of the block table (-1: past the context), and whether that is a page of the cache.
+__device__ __forceinline__ int key_entry(const KeyWeightParams &p, const int32_t *trow, int key, int n, int &slot) {
   const int b = p.block_size == 1 ? key : fast_div(key, p.bs_magic, p.bs_shift);
-  const int blk = key < n ? trow[b] : -1;
   slot = key - b * p.block_size;
+  return key < n ? trow[b] : -1;
+}
+__device__ __forceinline__ int as_page(const KeyWeightParams &p, int blk) {
   return (uint32_t)blk < (uint32_t)p.num_blocks ? blk : -1;
 }
 
-// The lane's half h of a key's codes, and its scale (log2 units; of code - 8 over 16) and zero point; zeros for page -1.
+// The lane's half h of a key's codes, and its word; zeros for page -1.
 template <int HS, int FMT>
 __device__ __forceinline__ void load_key(const KeyWeightParams &p, int blk, int slot, int kvh, int h,
-                                         uint32_t (&raw)[KwShape<HS, FMT>::kRaw], float &a, float &z) {
+                                         uint32_t (&raw)[KwShape<HS, FMT>::kRaw], uint32_t &word) {
   using Sh = KwShape<HS, FMT>;
-  a = z = 0.f;
+  word = 0;
 #pragma unroll
   for (int i = 0; i < Sh::kRaw; ++i) raw[i] = 0;
   if (blk < 0) return;
@@ -142,13 +145,17 @@ __device__ __forceinline__ void load_key(const KeyWeightParams &p, int blk, int 
 #pragma unroll
     for (int j = 0; j < 4; ++j) raw[4 * i + j] = x[j];
   }
-  const uint32_t word = p.words[blk * p.ws0 + slot * p.ws1 + kvh * p.ws2];
-  if constexpr (FMT == QP_CODES_INT4) {
-    a = __uint_as_float(word & 0xFFFFFFF0u) * (16.f * p.scale_log2);
-    z = ((float)(word & 0xFu) - 8.f) * 0.0625f;
-  } else {
-    a = __uint_as_float(word) * p.scale_log2;
-  }
+  word = p.words[blk * p.ws0 + slot * p.ws1 + kvh * p.ws2];
+}
+
+// A word's scale (log2 units; of code - 8 over 16) and zero point.
+template <int FMT>
+__device__ __forceinline__ float word_scale(const KeyWeightParams &p, uint32_t word) {
+  return FMT == QP_CODES_INT4 ? __uint_as_float(word & 0xFFFFFFF0u) * (16.f * p.scale_log2) : __uint_as_float(word) * p.scale_log2;
+}
+template <int FMT>
+__device__ __forceinline__ float word_zero(uint32_t word) {
+  return FMT == QP_CODES_INT4 ? ((float)(word & 0xFu) - 8.f) * 0.0625f : 0.f;
 }
 
 // Step i's 8 channels of the codes.
@@ -187,11 +194,10 @@ __global__ __launch_bounds__(kKwThreads) void key_scores_kernel(const KeyWeightP
   int blk[kKwSubs], slot[kKwSubs];
 #pragma unroll
   for (int s = 0; s < kKwSubs; ++s)
-    blk[s] = s < p.subs ? key_page(p, trow, k0 + 32 * (s * kKwWaves + w) + col, n, slot[s]) : -1;
+    blk[s] = s < p.subs ? as_page(p, key_entry(p, trow, k0 + 32 * (s * kKwWaves + w) + col, n, slot[s])) : -1;
   constexpr int kBuf = HS == 512 ? 1 : 2;
-  uint32_t raw[kBuf][Sh::kRaw];
-  float a[kBuf], z[kBuf];
-  load_key<HS, FMT>(p, blk[0], slot[0], kvh, h, raw[0], a[0], z[0]);
+  uint32_t raw[kBuf][Sh::kRaw], word[kBuf];
+  load_key<HS, FMT>(p, blk[0], slot[0], kvh, h, raw[0], word[0]);
   for (int r = tid / Sh::kGroup; r < 32; r += kKwThreads / Sh::kGroup) {
     float x;
     *reinterpret_cast<u32x4_t *>(qrows + r * Sh::kRowBytes + 16 * Sh::swz(r, tid % Sh::kGroup)) =
@@ -219,8 +225,9 @@ __global__ __launch_bounds__(kKwThreads) void key_scores_kernel(const KeyWeightP
     const int kw = k0 + 32 * (s * kKwWaves + w);
     if (s >= p.subs || kw >= n) break;
     const int cur = s % kBuf;
-    if (kBuf == 2 && s + 1 < kKwSubs) load_key<HS, FMT>(p, blk[s + 1], slot[s + 1], kvh, h, raw[(s + 1) % kBuf], a[(s + 1) % kBuf], z[(s + 1) % kBuf]);
-    if (kBuf == 1 && s > 0) load_key<HS, FMT>(p, blk[s], slot[s], kvh, h, raw[0], a[0], z[0]);
+    if (kBuf == 2 && s + 1 < kKwSubs) load_key<HS, FMT>(p, blk[s + 1], slot[s + 1], kvh, h, raw[(s + 1) % kBuf], word[(s + 1) % kBuf]);
+    if (kBuf == 1 && s > 0) load_key<HS, FMT>(p, blk[s], slot[s], kvh, h, raw[0], word[0]);
+    const float a = word_scale<FMT>(p, word[cur]), z = word_zero<FMT>(word[cur]);
     f32x16_t d = {};
 #pragma unroll
     for (int i = 0; i < Sh::kSteps; ++i)
@@ -230,7 +237,7 @@ __global__ __launch_bounds__(kKwThreads) void key_scores_kernel(const KeyWeightP
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int r = 8 * (i >> 2) + 4 * h + (i & 3);
-      float x = (FMT == QP_CODES_INT4 ? fmaf(-sum[i], z[cur], d[i]) : d[i]) * a[cur];
+      float x = (FMT == QP_CODES_INT4 ? fmaf(-sum[i], z, d[i]) : d[i]) * a;
       if (key > pos[i] || blk[s] < 0) x = -INFINITY;
       if (r < nrows && key < n) scores[r * p.score_stride + key] = x;
       const float to = fmaxf(m[i], x);
@@ -259,17 +266,18 @@ __global__ __launch_bounds__(kKwThreads) void key_scores_kernel(const KeyWeightP
   }
 }
 
-// A row's maximum and sum over the segments that a context has, in every lane of a wave.
-__device__ __forceinline__ float2 join_row(const float2 *part, int64_t stride, int used, int lane) {
+// A row's maximum and sum over the segments that a context has, in every one of a group of LANES lanes.
+template <int LANES>
+__device__ __forceinline__ float2 join_row(const float2 *part, int64_t stride, int used) {
   float top = kKwNone, l = 0.f;
-  for (int s = lane; s < used; s += 64) {
+  for (int s = threadIdx.x % LANES; s < used; s += LANES) {
     const float2 x = part[s * stride];
     const float to = fmaxf(top, x.x);
     l = fmaf(l, __builtin_amdgcn_exp2f(top - to), x.y * __builtin_amdgcn_exp2f(x.x - to));
     top = to;
   }
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
+  for (int o = 1; o < LANES; o <<= 1) {
     const float ot = shfl_xor_f(top, o), ol = shfl_xor_f(l, o);
     const float to = fmaxf(top, ot);
     l = l * __builtin_amdgcn_exp2f(top - to) + ol * __builtin_amdgcn_exp2f(ot - to);
@@ -306,7 +314,7 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(const KeyWeightPar
   };
   load(0);  // (in flight while the statistics are joined)
   for (int r = tid >> 6; r < nrows; r += 4) {
-    const float2 st = join_row(p.part + head * p.segments * p.max_rows + r, p.max_rows, used, lane);
+    const float2 st = join_row<64>(p.part + head * p.segments * p.max_rows + r, p.max_rows, used);
     if (lane == 0) stat[r] = st;
   }
   __syncthreads();
@@ -373,6 +381,9 @@ struct KwMany {
   using Sh = KwShape<HS, FMT>;
   static constexpr int kAt = HS <= 128 ? 2 : 1;        // 32-key tiles of a wave: each query operand serves them all
   static constexpr int kKeys = kAt * kKwWaves * 32;    // keys of a workgroup
+  // Whether a block's codes come during the one before: where the registers hold both (41 sequences of 4096 int4 keys, 64
+  // rows, head 128: 156 us so, 172 without; int8 at 128 would spill, and at 512 leave one wave per SIMD).
+  static constexpr bool kAhead = kAt * (Sh::kRaw + 4 * Sh::kSteps) <= 80;
   static constexpr int kStageRows = HS == 512 ? 32 : 64;
   static constexpr int kSumsAt = kStageRows * Sh::kRowBytes;
   static constexpr int kStage = kSumsAt + kStageRows * 16;
@@ -380,7 +391,7 @@ struct KwMany {
 };
 
 template <int HS, int FMT, int PASS>
-__global__ __launch_bounds__(kKwThreads, HS <= 256 ? 2 : 1) void key_weights_kernel(const KeyWeightParams p) {
+__global__ __launch_bounds__(kKwThreads, 2) void key_weights_kernel(const KeyWeightParams p) {
   using Sh = KwShape<HS, FMT>;
   using Mn = KwMany<HS, FMT>;
   constexpr int kAt = Mn::kAt, kTiles = Mn::kStageRows / 32;
@@ -393,19 +404,26 @@ __global__ __launch_bounds__(kKwThreads, HS <= 256 ? 2 : 1) void key_weights_ker
   const int segment = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
   const int G = p.num_q_heads / p.num_kv_heads;
   const int n = max(0, min(p.used_k[seq], p.max_keys));
-  const int k0 = segment * Mn::kKeys;
-  if (k0 >= n) return;
+  const int blocks = min(p.subs, (n + Mn::kKeys - 1) / Mn::kKeys - segment * p.subs);  // blocks of kKeys keys
+  if (blocks <= 0) return;
   const int q0 = max(0, p.cu_q[seq]), qlen = max(0, min(p.cu_q[seq + 1], p.num_tokens) - q0);
   const int nrows = min(qlen * G, p.max_rows), before = n - qlen;  // row r's token sees the keys up to before + r / G
   const int64_t head = (int64_t)seq * p.num_kv_heads + kvh;
   const int32_t *trow = p.table + (int64_t)seq * p.table_stride;
-  // A stage's rows go through HBM -> LDS copies: copy i of a wave fills units 64 (w + 4 i) .., the swizzle in the source.
+  // The rows go by in stages, once for each block of keys: step g is stage g % stages for block g / stages. Up to two stages
+  // stay where they are. A stage comes by HBM -> LDS copies: copy i of a wave fills units 64 (w + 4 i) .., the swizzle in
+  // the source.
+  const int stages = (nrows + Mn::kStageRows - 1) / Mn::kStageRows, ntiles = (nrows + 31) / 32;
+  const bool stay = stages <= 2;
+  const int steps = blocks * stages;
   const uint32_t lds0 = lds_addr(smem);
   const uint8_t *rows = reinterpret_cast<const uint8_t *>(p.rows) + head * p.row_cap * Sh::kRowBytes;
   const uint8_t *sums = reinterpret_cast<const uint8_t *>(p.sums) + head * p.row_cap * 16;
   const uint8_t *stats = reinterpret_cast<const uint8_t *>(p.stat) + head * p.row_cap * 8;
-  auto copy = [&](int st) {
-    const uint32_t dst = lds0 + (uint32_t)((st & 1) * Mn::kStage);
+  auto copy = [&](int g) {
+    if (g >= steps || (stay && g >= stages)) return;
+    const int st = g % stages;
+    const uint32_t dst = lds0 + (uint32_t)((g & 1) * Mn::kStage);
 #pragma unroll
     for (int i = 0; i < Mn::kCopies; ++i) {
       const int at = 64 * (w + kKwWaves * i), d = at + lane, r = d / Sh::kGroup, c = d % Sh::kGroup;
@@ -415,183 +433,216 @@ __global__ __launch_bounds__(kKwThreads, HS <= 256 ? 2 : 1) void key_weights_ker
     if (FMT == QP_CODES_INT4 && w == 0 && lane < Mn::kStageRows)
       dma16_saddr<false>(sums + (int64_t)st * Mn::kStageRows * 16, 16u * lane, dst + Mn::kSumsAt);
     if (PASS == 2 && w == 1 && lane < Mn::kStageRows / 2)
-      dma16_saddr<false>(stats + (int64_t)st * Mn::kStageRows * 8, 16u * lane, lds_addr(&state[st % 3][0][0]));
+      dma16_saddr<false>(stats + (int64_t)st * Mn::kStageRows * 8, 16u * lane, lds_addr(&state[g % 3][0][0]));
   };
-  const int stages = (nrows + Mn::kStageRows - 1) / Mn::kStageRows;
-  if (stages > 0) copy(0);
-
-  // ---- the lane's keys, half h of their channels; a key past the context, or on a page that does not exist, is not seen
-  const int kw = k0 + 32 * kAt * w;  // the wave's keys kw ..
-  u32x4_t kop[kAt][Sh::kSteps], kz[kAt];
-  float a[kAt];
-  bool ok[kAt], all = true;
-#pragma unroll
-  for (int k = 0; k < kAt; ++k) {
-    int slot;
-    const int blk = key_page(p, trow, kw + 32 * k + col, n, slot);
-    ok[k] = blk >= 0;
-    all &= ok[k];
-    uint32_t raw[Sh::kRaw];
-    float z;
-    load_key<HS, FMT>(p, blk, slot, kvh, h, raw, a[k], z);
-    kz[k] = zero_operand(z, h);
-#pragma unroll
-    for (int i = 0; i < Sh::kSteps; ++i) kop[k][i] = key_operand<HS, FMT>(raw, i);
-    // (a key that is not there has the scale NaN, which no stored one has)
-    if (PASS == 1 && h == 0) kscale[w][32 * k + col] = ok[k] ? a[k] : __builtin_nanf("");
-  }
-  all = __all(all);
-  wave_sync();
-  f32x4_t av[PASS == 1 ? kAt : 1][4];  // (first pass) the scales of the lane's keys 8 q + 4 h .. of each tile
-  if constexpr (PASS == 1) {
+  copy(0);
+  // the lane's keys, half h of their channels: a block's codes are loaded while the one before is at work, its table entries
+  // one block earlier. A key past the context, or on a page that does not exist, is not seen.
+  int entry[kAt], slot[kAt];
+  uint32_t raw[kAt][Sh::kRaw], word[kAt];
+  uint32_t there = 0;
+  const int first = segment * p.subs * Mn::kKeys + 32 * kAt * w;  // the wave's keys of a block: first + kKeys block ..
+  auto entries = [&](int blk) {
 #pragma unroll
     for (int k = 0; k < kAt; ++k)
+      entry[k] = blk < blocks ? key_entry(p, trow, first + Mn::kKeys * blk + 32 * k + col, n, slot[k]) : -1;
+  };
+  auto codes = [&]() {
+    there = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) av[k][q] = *reinterpret_cast<const f32x4_t *>(&kscale[w][32 * k + 8 * q + 4 * h]);
+    for (int k = 0; k < kAt; ++k) {
+      const int page = as_page(p, entry[k]);
+      there |= page >= 0 ? 1u << k : 0u;
+      load_key<HS, FMT>(p, page, slot[k], kvh, h, raw[k], word[k]);
+    }
+  };
+  entries(0);
+  if (Mn::kAhead) {
+    codes();
+    entries(1);
   }
-  float sum[kAt];
-  int first_row[kAt];  // (second pass) the first row whose token sees the lane's key
-#pragma unroll
-  for (int k = 0; k < kAt; ++k) {
-    sum[k] = 0.f;
-    first_row[k] = max(0, kw + 32 * k + col - before) * G;
-  }
-  // (first pass) a stage's statistics of the four waves, joined when all of them are there
-  auto join = [&](int st) {
-    const int r = st * Mn::kStageRows + tid;
-    if (st < 0 || tid >= Mn::kStageRows || r >= nrows) return;
+
+  u32x4_t kop[kAt][Sh::kSteps], kz[kAt];
+  float a[kAt], sum[kAt];
+  int first_row[kAt];                          // (second pass) the first row whose token sees the lane's key
+  f32x4_t av[PASS == 1 ? kAt : 1][4];          // (first pass) the scales of the lane's keys 8 q + 4 h .. of each tile
+  f32x16_t d[kAt], dn[kAt];
+  // (first pass) a step's statistics of the four waves, joined when all of them are there
+  auto join = [&](int g) {
+    if (g < 0) return;
+    const int r = g % stages * Mn::kStageRows + tid;
+    if (tid >= Mn::kStageRows || r >= nrows) return;
     float to = kKwNone, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < kKwWaves; ++i) to = fmaxf(to, state[st % 3][i][tid].x);
+    for (int i = 0; i < kKwWaves; ++i) to = fmaxf(to, state[g % 3][i][tid].x);
 #pragma unroll
-    for (int i = 0; i < kKwWaves; ++i) l = fmaf(state[st % 3][i][tid].y, __builtin_amdgcn_exp2f(state[st % 3][i][tid].x - to), l);
-    p.part[(head * p.segments + segment) * p.max_rows + r] = make_float2(to, l);
+    for (int i = 0; i < kKwWaves; ++i) l = fmaf(state[g % 3][i][tid].y, __builtin_amdgcn_exp2f(state[g % 3][i][tid].x - to), l);
+    p.part[(head * p.segments + segment * p.subs + g / stages) * p.max_rows + r] = make_float2(to, l);
   };
-  auto scores = [&](int tile, f32x16_t (&d)[kAt]) {
-    const uint8_t *stage = smem + (tile / kTiles & 1) * Mn::kStage;
-    const int t = tile % kTiles;
+  for (int blk = 0; blk < blocks; ++blk) {
+    const int kw = first + Mn::kKeys * blk, g0 = blk * stages;
+    bool ok[kAt];
+    if (!Mn::kAhead) codes();
 #pragma unroll
-    for (int k = 0; k < kAt; ++k) d[k] = f32x16_t{};
-    if constexpr (FMT == QP_CODES_INT4) {
-      const u32x4_t q = *reinterpret_cast<const u32x4_t *>(stage + Mn::kSumsAt + 16 * (32 * t + col));
+    for (int k = 0; k < kAt; ++k) {
+      ok[k] = there >> k & 1;
+      a[k] = word_scale<FMT>(p, word[k]);
+      kz[k] = zero_operand(word_zero<FMT>(word[k]), h);
 #pragma unroll
-      for (int k = 0; k < kAt; ++k) d[k] = PASS == 1 ? kw_mfma(kz[k], q, d[k]) : kw_mfma(q, kz[k], d[k]);
+      for (int i = 0; i < Sh::kSteps; ++i) kop[k][i] = key_operand<HS, FMT>(raw[k], i);
+      // (a key that is not there has the scale NaN, which no stored one has)
+      if (PASS == 1 && h == 0) kscale[w][32 * k + col] = ok[k] ? a[k] : __builtin_nanf("");
+      sum[k] = 0.f;
+      first_row[k] = max(0, kw + 32 * k + col - before) * G;
     }
-#pragma unroll
-    for (int i = 0; i < Sh::kSteps; ++i) {
-      const u32x4_t q = *reinterpret_cast<const u32x4_t *>(stage + (32 * t + col) * Sh::kRowBytes + 16 * Sh::swz(col, Sh::unit(h, i)));
-#pragma unroll
-      for (int k = 0; k < kAt; ++k) d[k] = PASS == 1 ? kw_mfma(kop[k][i], q, d[k]) : kw_mfma(q, kop[k][i], d[k]);
-    }
-  };
-  // a tile's scores to statistics, or weights. MASK: some row does not see all of the wave's keys, or some are not there
-  auto process = [&](int tile, f32x16_t (&d)[kAt], auto mask_tag) {
-    constexpr bool MASK = decltype(mask_tag)::value;
-    const int st = tile / kTiles, t = tile % kTiles, r0 = 32 * tile;
+    const bool all = __all(there == (1u << kAt) - 1);
+    const uint32_t shown = there;
     if constexpr (PASS == 1) {
-      // lane: row r0 + col, keys 8 (i / 4) + 4 h + i % 4 of each tile
-      float top = kKwNone, l = 0.f;
-      const int pos = MASK ? before + (r0 + col) / G : 0;
+      wave_sync();
 #pragma unroll
       for (int k = 0; k < kAt; ++k)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float sc = av[k][i >> 2][i & 3];
-          d[k][i] *= sc;
-          if (MASK && (kw + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3) > pos || sc != sc)) d[k][i] = -INFINITY;
-          top = fmaxf(top, d[k][i]);
-        }
-      {
-        const uint32_t b = __float_as_uint(top);
-        const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-        top = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+        for (int q = 0; q < 4; ++q) av[k][q] = *reinterpret_cast<const f32x4_t *>(&kscale[w][32 * k + 8 * q + 4 * h]);
+      wave_sync();
+    }
+    if (blk == 0) {
+      wait_vmcnt<0>();
+      __syncthreads();
+      copy(1);
+    }
+    if (Mn::kAhead) codes();
+    entries(blk + (Mn::kAhead ? 2 : 1));
+    auto scores = [&](int tile, f32x16_t (&d)[kAt]) {
+      const int st = tile / kTiles, t = tile % kTiles;
+      const uint8_t *stage = smem + ((stay ? st : g0 + st) & 1) * Mn::kStage;
+#pragma unroll
+      for (int k = 0; k < kAt; ++k) d[k] = f32x16_t{};
+      if constexpr (FMT == QP_CODES_INT4) {
+        const u32x4_t q = *reinterpret_cast<const u32x4_t *>(stage + Mn::kSumsAt + 16 * (32 * t + col));
+#pragma unroll
+        for (int k = 0; k < kAt; ++k) d[k] = PASS == 1 ? kw_mfma(kz[k], q, d[k]) : kw_mfma(q, kz[k], d[k]);
       }
 #pragma unroll
-      for (int k = 0; k < kAt; ++k)
+      for (int i = 0; i < Sh::kSteps; ++i) {
+        const u32x4_t q = *reinterpret_cast<const u32x4_t *>(stage + (32 * t + col) * Sh::kRowBytes + 16 * Sh::swz(col, Sh::unit(h, i)));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(d[k][i] - top);
-      {
-        const uint32_t b = __float_as_uint(l);
-        const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-        l = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+        for (int k = 0; k < kAt; ++k) d[k] = PASS == 1 ? kw_mfma(kop[k][i], q, d[k]) : kw_mfma(q, kop[k][i], d[k]);
       }
-      if (h == 0) state[st % 3][w][32 * t + col] = make_float2(top, l);
-    } else {
-      // lane: key col of each tile, rows r0 + 8 q + 4 h + j
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4_t *sp = reinterpret_cast<const f32x4_t *>(&state[st % 3][0][32 * t + 8 * q + 4 * h]);
-        const f32x4_t s0 = sp[0], s1 = sp[1];
-        const float mx[4] = {s0[0], s0[2], s1[0], s1[2]}, iv[4] = {s0[1], s0[3], s1[1], s1[3]};
+    };
+    // a tile's scores to statistics, or weights. MASK: some row does not see all of the wave's keys, or some are not there
+    auto process = [&](int tile, f32x16_t (&d)[kAt], auto mask_tag) {
+      constexpr bool MASK = decltype(mask_tag)::value;
+      const int t = tile % kTiles, r0 = 32 * tile, at = PASS == 2 && stay ? tile / kTiles : (g0 + tile / kTiles) % 3;
+      if constexpr (PASS == 1) {
+        // lane: row r0 + col, keys 8 (i / 4) + 4 h + i % 4 of each tile
+        float top = kKwNone, l = 0.f;
+        const int pos = MASK ? before + (r0 + col) / G : 0;
 #pragma unroll
         for (int k = 0; k < kAt; ++k)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float e = __builtin_amdgcn_exp2f(fmaf(d[k][4 * q + j], a[k], -mx[j]));
-            if (MASK && r0 + 8 * q + 4 * h + j < first_row[k]) e = 0.f;
-            sum[k] = fmaf(e, iv[j], sum[k]);
+          for (int i = 0; i < 16; ++i) {
+            const float sc = av[k][i >> 2][i & 3];
+            d[k][i] *= sc;
+            if (MASK && (kw + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3) > pos || sc != sc)) d[k][i] = -INFINITY;
+            top = fmaxf(top, d[k][i]);
           }
+        {
+          const uint32_t b = __float_as_uint(top);
+          const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+          top = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+        }
+#pragma unroll
+        for (int k = 0; k < kAt; ++k)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(d[k][i] - top);
+        {
+          const uint32_t b = __float_as_uint(l);
+          const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+          l = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+        }
+        if (h == 0) state[at][w][32 * t + col] = make_float2(top, l);
+      } else {
+        // lane: key col of each tile, rows r0 + 8 q + 4 h + j
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4_t *sp = reinterpret_cast<const f32x4_t *>(&state[at][0][32 * t + 8 * q + 4 * h]);
+          const f32x4_t s0 = sp[0], s1 = sp[1];
+          const float mx[4] = {s0[0], s0[2], s1[0], s1[2]}, iv[4] = {s0[1], s0[3], s1[1], s1[3]};
+#pragma unroll
+          for (int k = 0; k < kAt; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float e = __builtin_amdgcn_exp2f(fmaf(d[k][4 * q + j], a[k], -mx[j]));
+              if (MASK && r0 + 8 * q + 4 * h + j < first_row[k]) e = 0.f;
+              sum[k] = fmaf(e, iv[j], sum[k]);
+            }
+        }
       }
-    }
-  };
+    };
 
-  // ---- the walk over the rows' tiles: one's scores are made beside the one before's exponentials. Before a stage's last
-  // tile the waves meet: the next stage has landed, every wave is past this one's rows, and the one after takes their place.
-  const int ntiles = stages * kTiles;
-  wait_vmcnt<0>();
-  __syncthreads();
-  if (stages > 1) copy(1);
-  f32x16_t d[kAt], dn[kAt];
-  if (ntiles > 0) scores(0, d);
-  auto step = [&](int tile, auto mask_tag) {
-    const int st = tile / kTiles;
-    if (tile % kTiles == kTiles - 1 && st + 1 < stages) {
-      wait_vmcnt<0>();
-      __syncthreads();
-      if (st + 2 < stages) copy(st + 2);
-      if (PASS == 1) join(st - 1);
+    // ---- the walk over the rows' tiles: one's scores are made beside the one before's exponentials. Before a stage's last
+    // tile the waves meet: the next stage has landed, every wave is past this one's rows, and the one after takes their place.
+    auto meet = [&](int tile) {
+      if (tile != ntiles - 1 && tile % kTiles != kTiles - 1) return;
+      const int g = g0 + tile / kTiles;
+      if (g + 1 < steps) {
+        wait_vmcnt<0>();
+        __syncthreads();
+        copy(g + 2);
+        if (PASS == 1) join(g - 1);
+      }
+    };
+    // later rows see more: from `whole` on every row of a tile sees all of the wave's keys
+    const int64_t ahead = (int64_t)max(0, kw + 32 * kAt - 1 - before) * G;
+    const int whole = uniform(all ? (int)min((int64_t)ntiles, (ahead + 31) / 32) : ntiles);
+    if (ntiles > 0) scores(0, d);
+    auto step = [&](int tile, auto mask_tag) {
+      meet(tile);
+      scores(tile + 1, dn);
+      process(tile, d, mask_tag);
+#pragma unroll
+      for (int k = 0; k < kAt; ++k) d[k] = dn[k];
+    };
+    int tile = 0;
+    for (; tile < min(whole, ntiles - 1); ++tile) step(tile, std::true_type{});
+    for (; tile < ntiles - 1; ++tile) step(tile, std::false_type{});
+    if (ntiles > 0) {
+      meet(tile);
+      if (tile < whole) process(tile, d, std::true_type{});
+      else process(tile, d, std::false_type{});
     }
-    scores(tile + 1, dn);  // (the last tile's next one is not used: whatever lies in its place)
-    process(tile, d, mask_tag);
+    if constexpr (PASS == 2) {
 #pragma unroll
-    for (int k = 0; k < kAt; ++k) d[k] = dn[k];
-  };
-  // later rows see more: from `whole` on every row of a tile sees all of the wave's keys
-  const int64_t ahead = (int64_t)max(0, kw + 32 * kAt - 1 - before) * G;
-  const int whole = uniform(all ? (int)min((int64_t)ntiles, (ahead + 31) / 32) : ntiles);
-  int tile = 0;
-  for (; tile < whole; ++tile) step(tile, std::true_type{});
-  for (; tile < ntiles; ++tile) step(tile, std::false_type{});
-  if constexpr (PASS == 1) {
-    __syncthreads();
-    join(stages - 2);
-    join(stages - 1);
-  } else {
-#pragma unroll
-    for (int k = 0; k < kAt; ++k) {
-      const int key = kw + 32 * k + col;
-      const float x = sum[k] + shfl_xor_f(sum[k], 32);
-      if (h == 0 && key < n) {
-        float v = ok[k] ? x : 0.f;
-        if (p.prev) v = fmaf(p.decay, p.prev[(int64_t)seq * p.ps0 + (int64_t)kvh * p.ps1 + key], v);
-        p.out[(int64_t)seq * p.os0 + (int64_t)kvh * p.os1 + key] = v;
+      for (int k = 0; k < kAt; ++k) {
+        const int key = kw + 32 * k + col;
+        const float x = sum[k] + shfl_xor_f(sum[k], 32);
+        if (h == 0 && key < n) {
+          float v = shown >> k & 1 ? x : 0.f;
+          if (p.prev) v = fmaf(p.decay, p.prev[(int64_t)seq * p.ps0 + (int64_t)kvh * p.ps1 + key], v);
+          p.out[(int64_t)seq * p.os0 + (int64_t)kvh * p.os1 + key] = v;
+        }
       }
     }
   }
+  if (PASS == 1 && steps > 0) {
+    __syncthreads();
+    join(steps - 2);
+    join(steps - 1);
+  }
 }
 
-// A row's maximum and sum over all segments, a wave per row.
+// A row's maximum and sum over all segments, LANES lanes per row.
+template <int LANES>
 __global__ __launch_bounds__(256) void key_weights_join_kernel(const KeyWeightParams p) {
-  const int lane = threadIdx.x & 63;
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y, seq = blockIdx.z;
-  if (row >= p.row_cap) return;
+  const int row = (blockIdx.x * 256 + threadIdx.x) / LANES, kvh = blockIdx.y, seq = blockIdx.z;
   const int G = p.num_q_heads / p.num_kv_heads;
   const int q0 = max(0, p.cu_q[seq]), qlen = max(0, min(p.cu_q[seq + 1], p.num_tokens) - q0);
   const int n = max(0, min(p.used_k[seq], p.max_keys)), used = (n + p.seg_keys - 1) / p.seg_keys;
   const int64_t head = (int64_t)seq * p.num_kv_heads + kvh;
+  if (row >= p.row_cap) return;  // (whole groups)
   float2 st = make_float2(0.f, 0.f);  // (a row that pads a stage has no share)
-  if (row < min(qlen * G, p.max_rows)) st = join_row(p.part + head * p.segments * p.max_rows + row, p.max_rows, used, lane);
-  if (lane == 0) p.stat[head * p.row_cap + row] = st;
+  if (row < min(qlen * G, p.max_rows)) st = join_row<LANES>(p.part + head * p.segments * p.max_rows + row, p.max_rows, used);
+  if (threadIdx.x % LANES == 0) p.stat[head * p.row_cap + row] = st;
 }
 
 struct KwPlan {
@@ -620,6 +671,9 @@ KwPlan kw_plan(const qp_key_weights_args *a) {
   } else {
     k.seg_keys = many_keys(a->head_size);
     k.row_cap = (int)((k.max_rows + 63) / 64 * 64);
+    const int64_t blocks = (keys + k.seg_keys - 1) / k.seg_keys;
+    k.subs = kKwBlocks;  // several blocks, as long as two workgroups per CU are there
+    while (k.subs > 1 && heads * ((blocks + k.subs - 1) / k.subs) < 2 * cus) k.subs >>= 1;
   }
   k.segments = (int)((keys + k.seg_keys - 1) / k.seg_keys);
   k.part_bytes = (heads * k.segments * k.max_rows * 8 + 255) / 256 * 256;
@@ -635,7 +689,7 @@ KwPlan kw_plan(const qp_key_weights_args *a) {
 
 template <int HS, int FMT>
 void launch_key_weights(KeyWeightParams &p, int seqs, hipStream_t s) {
-  const dim3 grid(p.segments, p.num_kv_heads, seqs);
+  const dim3 grid(p.scores ? p.segments : (p.segments + p.subs - 1) / p.subs, p.num_kv_heads, seqs);
   if (p.scores) {
     if (p.max_rows <= 8) key_scores_kernel<HS, FMT, 4><<<grid, kKwThreads, 0, s>>>(p);
     else if (p.max_rows <= 16) key_scores_kernel<HS, FMT, 8><<<grid, kKwThreads, 0, s>>>(p);
@@ -647,7 +701,9 @@ void launch_key_weights(KeyWeightParams &p, int seqs, hipStream_t s) {
     const int per = kKwThreads / KwShape<HS, FMT>::kGroup;
     key_weights_rows_kernel<HS, FMT><<<dim3(p.row_cap / per, p.num_kv_heads, seqs), kKwThreads, 0, s>>>(p);
     key_weights_kernel<HS, FMT, 1><<<grid, kKwThreads, 0, s>>>(p);
-    key_weights_join_kernel<<<dim3(p.row_cap / 4, p.num_kv_heads, seqs), 256, 0, s>>>(p);
+    // (lanes by the segments: 8 of them, 480 heads of 256 rows: 5 us with 4 lanes, 33 with 64)
+    if (p.segments > 32) key_weights_join_kernel<64><<<dim3(p.row_cap / 4, p.num_kv_heads, seqs), 256, 0, s>>>(p);
+    else key_weights_join_kernel<4><<<dim3(p.row_cap / 64, p.num_kv_heads, seqs), 256, 0, s>>>(p);
   }
   key_weights_kernel<HS, FMT, 2><<<grid, kKwThreads, 0, s>>>(p);
 }
