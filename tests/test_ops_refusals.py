@@ -256,3 +256,31 @@ def test_evict_keys_refusals(lib):
         evict_keys(kc, kc[..., :16], ks, ks, w, **kw)
     with pytest.raises(ValueError, match="weights must be"):
         evict_keys(kc, kc, ks, ks, w.double(), **kw)
+
+
+# ------------------------------------------------------------------------------------- sizes that a launch cannot take
+
+def test_refuses_sizes_past_the_launch_limits(lib):
+    big = dict(num_tokens=1 << 21, num_splits=2, workspace=4096, workspace_bytes=1 << 62)
+    assert lib.qp_prompt(prompt_args(**big), None) == -2 and "rows for splits" in lib.qp_last_error().decode()
+    assert lib.qp_prompt_workspace_size(prompt_args(**big)) == 0
+    assert lib.qp_prompt(prompt_args(num_tokens=1 << 28), None) == -2 and "rows" in lib.qp_last_error().decode()
+    assert lib.qp_key_weights(weight_args(max_query_len=1 << 23), None) == -2 and "rows" in lib.qp_last_error().decode()
+    long = (1 << 30) + 1
+    assert lib.qp_key_weights(weight_args(max_seqlen_k=long), None) == -2 and "positions" in lib.qp_last_error().decode()
+    assert lib.qp_key_weights_workspace_size(weight_args(max_seqlen_k=long)) == 0
+    assert lib.qp_evict(*evict_args(max_seqlen_k=long), None) == -2 and "positions" in lib.qp_last_error().decode()
+
+
+def test_refuses_gradients_and_moves_in_place(lib):
+    from vllm_quantpack.attention.eviction import evict_keys
+    from vllm_quantpack.attention.key_weights import key_weights
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    q, kc, ks = torch.zeros((1, 4, 64), dtype=torch.bfloat16), torch.zeros((6, 16, 2, 32), dtype=torch.uint8), torch.zeros((6, 16, 2))
+    table = i32([[0, 1, 2]])
+    with pytest.raises(NotImplementedError, match="backward"):
+        key_weights(q.requires_grad_(), kc, ks, torch.zeros((1, 2, 40)), cu_seqlens_q=i32([0, 1]), seqused_k=i32([40]),
+                    block_table=table, max_seqlen_q=1, softmax_scale=0.1)
+    with pytest.raises(ValueError, match="must not be block_table"):
+        evict_keys(kc, kc, ks, ks, torch.zeros((1, 2, 48)), seqused_k=i32([48]), block_table=table, new_block_table=table,
+                   budget=32)

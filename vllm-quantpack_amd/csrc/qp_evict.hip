@@ -550,6 +550,7 @@ int check_evict(const qp_paged_cache *c, const qp_evict_args *a) {
   QP_SUPPORTED((int64_t)c->num_blocks * c->block_size < (int64_t(1) << 31), "qp_evict: at most 2^31 - 1 cache slots");
   QP_REQUIRE(a->num_seqs >= 0 && a->max_seqlen_k >= 0 && a->max_blocks >= 0 && a->new_max_blocks >= 0, "qp_evict: bad sizes");
   QP_SUPPORTED(a->num_seqs < 65536 && c->num_kv_heads < 65536, "qp_evict: at most 65535 sequences and KV heads");
+  QP_SUPPORTED(a->max_seqlen_k <= 1 << 30, "qp_evict: at most 2^30 positions");
   QP_REQUIRE(a->budget > 0 && a->sinks >= 0 && a->recent >= 0 && (int64_t)a->sinks + a->recent <= a->budget,
              "qp_evict: the budget must be positive and hold the first `sinks` and the last `recent` positions");
   return QP_OK;

@@ -720,8 +720,9 @@ int check_key_weights(const qp_key_weights_args *a) {
              "qp_key_weights: bad sizes");
   QP_SUPPORTED(a->num_seqs < 65536 && a->num_kv_heads < 65536, "qp_key_weights: at most 65535 sequences and KV heads");
   const int64_t group = a->num_q_heads / a->num_kv_heads;
-  QP_SUPPORTED(a->max_query_len * group < (int64_t(1) << 30) && a->num_tokens * group < (int64_t(1) << 31),
-               "qp_key_weights: too many query rows");
+  QP_SUPPORTED(a->max_query_len * group < (int64_t(1) << 25) && a->num_tokens * group < (int64_t(1) << 31),
+               "qp_key_weights: too many query rows");  // (up to 64 threads for each of a sequence's)
+  QP_SUPPORTED(a->max_seqlen_k <= 1 << 30, "qp_key_weights: at most 2^30 positions");
   QP_REQUIRE(a->softmax_scale > 0.f && a->softmax_scale < INFINITY, "qp_key_weights: the softmax scale must be positive");
   return QP_OK;
 }

@@ -772,6 +772,9 @@ int check_prompt(const qp_prompt_args *a) {
              "qp_prompt: query heads must be a multiple of KV heads");
   QP_REQUIRE(a->num_splits >= 0 && a->num_splits <= 128, "qp_prompt: 0..128 splits");
   QP_REQUIRE(a->softmax_scale > 0.f && a->softmax_scale < INFINITY, "qp_prompt: the softmax scale must be positive");
+  const int64_t rows = (int64_t)a->num_tokens * a->num_q_heads;  // (the merge has up to 256 threads for each)
+  QP_SUPPORTED(rows < (int64_t(1) << 31) && a->num_kv_heads < 65536, "qp_prompt: too many rows");
+  QP_SUPPORTED(a->num_splits <= 1 || rows < (int64_t(1) << 24), "qp_prompt: too many rows for splits");
   return QP_OK;
 }
 
@@ -801,7 +804,6 @@ extern "C" int qp_prompt(const qp_prompt_args *a, qp_stream_t stream) {
   QP_SUPPORTED(a->key_stride[0] < (1 << 23) && a->value_stride[0] < (1 << 23), "qp_prompt: key rows more than 16 MiB apart");
   const int64_t rows = (int64_t)a->num_tokens * a->num_q_heads;
   const int64_t blocks = prompt_blocks(a);
-  QP_SUPPORTED(rows < (int64_t(1) << 31) && a->num_kv_heads < 65536, "qp_prompt: too many rows");
   int splits = prompt_splits(a);
   if (splits > 1 && (!a->workspace || a->workspace_bytes < prompt_partial_bytes(a, splits))) {
     QP_REQUIRE(a->num_splits == 0, "qp_prompt: workspace too small for the requested splits");

@@ -65,6 +65,8 @@ def evict_keys(k_cache, v_cache, k_scale_cache, v_scale_cache, weights, *, sequs
     _rows("new_weights", new_weights, torch.float32, seqs, nkv, budget)
     if new_seqused_k.dtype != torch.int32 or new_seqused_k.shape != (seqs,) or not new_seqused_k.is_contiguous():
         raise ValueError(f"evict_keys: new_seqused_k must be {seqs} contiguous int32 entries")
+    if seqs and block_table.numel() and new_block_table.data_ptr() == block_table.data_ptr():
+        raise ValueError("evict_keys: the kept cells move to other blocks: new_block_table must not be block_table")
     if seqs and (new_weights.data_ptr() == weights.data_ptr() or new_seqused_k.data_ptr() == seqused_k.data_ptr()):
         raise ValueError("evict_keys: weights and seqused_k are read while the new ones are written: give other tensors")
     _hip.same_device("evict_keys", k_cache, v_cache=v_cache, k_scale_cache=k_scale_cache, v_scale_cache=v_scale_cache,
