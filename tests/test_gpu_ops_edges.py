@@ -34,6 +34,16 @@ def test_prompt_groups_past_a_row_tile(device):
     run_prompt(device, [(3, 50)], 130, 1, 512, torch.bfloat16, seed=6)
 
 
+@pytest.mark.parametrize("dtype,causal", [("bf16", True), ("fp16", False)])
+def test_prompt_of_many_rows(device, dtype, causal):
+    """Enough rows, of enough sequences, for the larger row blocks; blocks that are full, and some with a row in them."""
+    import torch
+    rng = np.random.default_rng(11)
+    lens = [(int(t), int(t + n)) for t, n in zip(rng.integers(25, 50, 64), rng.integers(0, 90, 64))]
+    lens[3], lens[9], lens[20], lens[63] = (300, 333), (64, 64), (129, 100), (1, 77)
+    run_prompt(device, lens, 32, 8, 128, {"bf16": torch.bfloat16, "fp16": torch.float16}[dtype], causal=causal, seed=2)
+
+
 @pytest.mark.parametrize("hs,num_splits", [(128, 0), (512, 0), (64, 1)])
 def test_prompt_offsets_past_32_bits(device, hs, num_splits):
     """Key and value rows 64 Ki elements apart: the last ones lie 2^32 elements from the first."""

@@ -277,13 +277,12 @@ __device__ __forceinline__ void store_row(const PromptParams &p, const PromptBlo
 
 // ------------------------------------------------------------------------------------- heads of 64, 128 and 256
 
-template <int HS_, bool F16_>
+template <int HS_, bool F16_, int WAVES>
 struct PromptShape {
   static constexpr int HS = HS_;
   static constexpr bool F16 = F16_;
-  // Two waves per SIMD up to head 128, in one workgroup at 128, whose tiles then serve 256 rows, and in two at 64 (60 us
-  // against 63 on four sequences of up to 509 tokens over up to 4605 keys). At 256 a wave takes 512 registers.
-  static constexpr int kWaves = HS == 128 ? 8 : 4;
+  // Two waves per SIMD up to head 128, in one workgroup or two: prompt_rows says which. At 256 a wave takes 512 registers.
+  static constexpr int kWaves = WAVES;
   static constexpr int kWavesPerSimd = HS <= 128 ? 2 : 1;
   static constexpr int kThreads = kWaves * 64;
   static constexpr int kRows = kWaves * 32;
@@ -294,6 +293,8 @@ struct PromptShape {
   static constexpr int kOffV = kKRing * kTile;
   static constexpr int kLds = kOffV + kVRing * kTile;
   static constexpr int kCopies = kTile / 1024 / kWaves;  // 1 KiB copies of a wave, K and V each
+  static constexpr int kCopyRows = kWaves * 64 / kU;     // rows of copy i of all waves
+  static constexpr int kOffsets = kCopyRows >= 16 ? 1 : kCopies;
   static_assert(kTile % (1024 * kWaves) == 0 && kLds <= 160 * 1024, "LDS");
   // Position of unit c in row r of a K tile: 16 rows' reads of one unit hit every bank of the LDS once.
   static __host__ __device__ constexpr int k_swz(int r, int c) { return HS == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15); }
@@ -347,9 +348,10 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
     const uint8_t *kbase = reinterpret_cast<const uint8_t *>(p.k + (int64_t)(b.k0 + kb) * p.ks0 + (int64_t)b.kvh * p.ks1);
     const uint8_t *vbase = reinterpret_cast<const uint8_t *>(p.v + (int64_t)(b.k0 + kb) * p.vs0 + (int64_t)b.kvh * p.vs1);
     const uint32_t ksb = (uint32_t)(p.ks0 * 2), vsb = (uint32_t)(p.vs0 * 2);
-    uint32_t kvo[Sh::kCopies], vvo[Sh::kCopies];  // the lane's byte offsets in a whole tile
+    // the lane's byte offsets in a whole tile; copies a multiple of 16 rows apart differ by those rows only
+    uint32_t kvo[Sh::kOffsets], vvo[Sh::kOffsets];
 #pragma unroll
-    for (int i = 0; i < Sh::kCopies; ++i) {
+    for (int i = 0; i < Sh::kOffsets; ++i) {
       const int d = 64 * (w + Sh::kWaves * i) + lane, r = d / U, c = d % U;
       kvo[i] = (uint32_t)r * ksb + 16u * (uint32_t)Sh::k_swz(r, c);
       vvo[i] = (uint32_t)r * vsb + 16u * (uint32_t)Sh::v_swz(r, c);
@@ -360,14 +362,18 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
 #pragma unroll
       for (int i = 0; i < Sh::kCopies; ++i) {
         const int at = 64 * (w + Sh::kWaves * i);
-        uint32_t ko = kvo[i], vo = vvo[i];
+        const int base = i / Sh::kOffsets * Sh::kOffsets * Sh::kCopyRows;
+        const uint8_t *kc = kt + (int64_t)base * ksb, *vc = vt + (int64_t)base * vsb;
+        uint32_t ko = kvo[i % Sh::kOffsets], vo = vvo[i % Sh::kOffsets];
         if (left < KT - 1) {
+          kc = kt;
+          vc = vt;
           const int d = at + lane, r = d / U, c = d % U, rs = min(r, left);
           ko = (uint32_t)rs * ksb + 16u * (uint32_t)Sh::k_swz(r, c);
           vo = (uint32_t)rs * vsb + 16u * (uint32_t)Sh::v_swz(r, c);
         }
-        dma16_saddr<false>(kt, ko, lds0 + (uint32_t)(kslot * Sh::kTile + 16 * at));
-        dma16_saddr<false>(vt, vo, lds0 + (uint32_t)(Sh::kOffV + vslot * Sh::kTile + 16 * at));
+        dma16_saddr<false>(kc, ko, lds0 + (uint32_t)(kslot * Sh::kTile + 16 * at));
+        dma16_saddr<false>(vc, vo, lds0 + (uint32_t)(Sh::kOffV + vslot * Sh::kTile + 16 * at));
       }
     };
     // ---- operands. A swizzle changes the low bits of a unit's place only: a few lane offsets serve all steps, with the rest
@@ -705,16 +711,24 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptParams p)
     p.lse[t * p.ls0 + head * p.ls1] = sum != 0.f ? (top + log2f(sum)) * (1.f / kLog2e) : -INFINITY;
 }
 
-template <int HS>
-constexpr int prompt_rows() { return PromptShape<HS, false>::kRows; }
-
-int prompt_block_rows(int hs) {
-  return hs == 64 ? prompt_rows<64>() : hs == 128 ? prompt_rows<128>() : hs == 256 ? prompt_rows<256>() : kPromptWideRows;
+// Rows of a workgroup's block.
+int prompt_rows(const qp_prompt_args *a) {
+  if (a->head_size == 512) return kPromptWideRows;
+  if (a->head_size != 128) return 128;
+  // Head 128: blocks of 256 rows, which share a tile's copies, where there are two for each CU, or where one wave has all rows
+  // and the copies are the work; else two workgroups of 128 rows per CU. 128 against 256 rows, us, 32 / 8 heads: one prompt of
+  // 1024 tokens 28 / 34, 2048 53 / 60, 4096 152 / 140, 16384 2030 / 1950; 64 prompts of up to 100, 16 / 16 heads, 28 / 35; one
+  // token over 65536 keys, 64 / 8 heads, 75 / 61. (Head 64: 60 in blocks of 128 on four turns of up to 509 tokens over up to
+  // 4605 keys, 63 in blocks of 256.)
+  const int64_t rows = (int64_t)a->num_tokens * (a->num_q_heads / a->num_kv_heads), seqs = a->num_seqs;
+  if (rows <= 32 * seqs) return 256;
+  if (rows <= 128 * seqs) return 128;
+  return std::max((rows + 255) / 256, seqs) * a->num_kv_heads >= 2 * device_cus() ? 256 : 128;
 }
 
 // Workgroups of one key split at most: sequence s owns row blocks [cu_q[s] G / R + s, cu_q[s + 1] G / R + s + 1) of R rows.
 int64_t prompt_blocks(const qp_prompt_args *a) {
-  return (int64_t)a->num_tokens * (a->num_q_heads / a->num_kv_heads) / prompt_block_rows(a->head_size) + a->num_seqs;
+  return (int64_t)a->num_tokens * (a->num_q_heads / a->num_kv_heads) / prompt_rows(a) + a->num_seqs;
 }
 
 // Key splits of a call: 1 where the row blocks alone fill the GPU, else about two workgroups per CU, of 256 keys at least.
@@ -722,7 +736,7 @@ constexpr int kPromptSplitKeys = 256;
 
 int prompt_splits(const qp_prompt_args *a) {
   if (a->num_splits > 0) return a->num_splits;
-  const int64_t cus = device_cus(), G = a->num_q_heads / a->num_kv_heads, rows = prompt_block_rows(a->head_size);
+  const int64_t cus = device_cus(), G = a->num_q_heads / a->num_kv_heads, rows = prompt_rows(a);
   const int64_t filled = ((int64_t)a->num_tokens * G + rows - 1) / rows;  // (every sequence has a block of its own, too)
   const int64_t wgs = (filled > a->num_seqs ? filled : a->num_seqs) * a->num_kv_heads;
   if (wgs >= cus) return 1;
@@ -743,22 +757,28 @@ int64_t prompt_partial_bytes(const qp_prompt_args *a, int splits) {
 }
 
 template <int HS, bool F16>
-void launch_prompt(const PromptParams &p, dim3 grid, hipStream_t s) {
+void launch_prompt(const PromptParams &p, int rows, dim3 grid, hipStream_t s) {
   const uint32_t share = prompt_share(grid.y * grid.z);
   grid.x = ((grid.x + (1u << share) - 1) >> share) << share;
-  if constexpr (HS == 512) prompt_wide_kernel<F16><<<grid, 256, 0, s>>>(p);
-  else prompt_kernel<PromptShape<HS, F16>><<<grid, PromptShape<HS, F16>::kThreads, 0, s>>>(p);
+  if constexpr (HS == 512) {
+    prompt_wide_kernel<F16><<<grid, 256, 0, s>>>(p);
+  } else if constexpr (HS == 128) {
+    if (rows == 256) prompt_kernel<PromptShape<HS, F16, 8>><<<grid, 512, 0, s>>>(p);
+    else prompt_kernel<PromptShape<HS, F16, 4>><<<grid, 256, 0, s>>>(p);
+  } else {
+    prompt_kernel<PromptShape<HS, F16, 4>><<<grid, 256, 0, s>>>(p);
+  }
   if (p.num_splits > 1) {
-    const int64_t rows = (int64_t)p.num_tokens * p.num_q_heads;
-    if (p.num_splits > 8) prompt_merge_kernel<HS, F16, 4><<<(unsigned)rows, 256, 0, s>>>(p);
-    else prompt_merge_kernel<HS, F16, 1><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(p);
+    const int64_t out_rows = (int64_t)p.num_tokens * p.num_q_heads;
+    if (p.num_splits > 8) prompt_merge_kernel<HS, F16, 4><<<(unsigned)out_rows, 256, 0, s>>>(p);
+    else prompt_merge_kernel<HS, F16, 1><<<(unsigned)((out_rows + 3) / 4), 256, 0, s>>>(p);
   }
 }
 
 template <int HS>
-void launch_prompt_type(const PromptParams &p, int dtype, dim3 grid, hipStream_t s) {
-  if (dtype == QP_DTYPE_F16) launch_prompt<HS, true>(p, grid, s);
-  else launch_prompt<HS, false>(p, grid, s);
+void launch_prompt_type(const PromptParams &p, int dtype, int rows, dim3 grid, hipStream_t s) {
+  if (dtype == QP_DTYPE_F16) launch_prompt<HS, true>(p, rows, grid, s);
+  else launch_prompt<HS, false>(p, rows, grid, s);
 }
 
 // What a call refuses.
@@ -840,11 +860,12 @@ extern "C" int qp_prompt(const qp_prompt_args *a, qp_stream_t stream) {
   p.min_keys = a->num_splits == 0 ? kPromptSplitKeys : 0;
   p.causal = a->causal != 0;
   p.scale_log2 = a->softmax_scale * kLog2e;
+  const int block_rows = prompt_rows(a);
   const dim3 grid((unsigned)blocks, a->num_kv_heads, splits);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (a->head_size == 64) launch_prompt_type<64>(p, a->dtype, grid, s);
-  else if (a->head_size == 128) launch_prompt_type<128>(p, a->dtype, grid, s);
-  else if (a->head_size == 256) launch_prompt_type<256>(p, a->dtype, grid, s);
-  else launch_prompt_type<512>(p, a->dtype, grid, s);
+  if (a->head_size == 64) launch_prompt_type<64>(p, a->dtype, block_rows, grid, s);
+  else if (a->head_size == 128) launch_prompt_type<128>(p, a->dtype, block_rows, grid, s);
+  else if (a->head_size == 256) launch_prompt_type<256>(p, a->dtype, block_rows, grid, s);
+  else launch_prompt_type<512>(p, a->dtype, block_rows, grid, s);
   return launch_status();
 }
