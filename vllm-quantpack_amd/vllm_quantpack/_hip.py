@@ -228,12 +228,14 @@ def stream_of(t: torch.Tensor):
 
 
 _NO_GUARD = contextlib.nullcontext()
+# (without the check that torch's GPU state is up, which a tensor on a GPU implies)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device_of(t: torch.Tensor):
     """A context in which t's device is the current one: a launch goes to the current device, whatever its stream."""
     index = t.get_device()
-    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _NO_GUARD if index == _current_device() else torch.cuda.device(index)
 
 
 def same_device(what: str, first: torch.Tensor, **tensors) -> None:

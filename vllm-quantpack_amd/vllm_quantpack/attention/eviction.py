@@ -21,7 +21,9 @@ def _table(name, t, seqs):
 
 
 def _rows(name, t, dtype, seqs, nkv, length):
-    if t.dtype != dtype or t.dim() != 3 or t.shape[:2] != (seqs, nkv) or t.shape[2] < length or t.stride(2) != 1:
+    shape = t.shape
+    if (t.dtype != dtype or len(shape) != 3 or shape[0] != seqs or shape[1] != nkv or shape[2] < length or
+            t.stride(2) != 1):
         raise ValueError(f"evict_keys: {name} must be {dtype} [{seqs}, {nkv}, {length} or more], contiguous in the last "
                          f"dimension, got {t.dtype} {tuple(t.shape)}")
 
@@ -40,11 +42,11 @@ def evict_keys(k_cache, v_cache, k_scale_cache, v_scale_cache, weights, *, sequs
     No host synchronisation; the workspace comes from torch's caching allocator."""
     if k_cache.dim() != 4 or v_cache.dim() != 4 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         raise ValueError("evict_keys: the cache views must be (blocks, slots, heads, bytes) with contiguous bytes")
-    seqs, nkv = seqused_k.shape[0], k_cache.shape[2]
-    hs = v_cache.shape[3] // 8 * 16  # (an int4 half's view may have its word's 4 bytes behind the codes)
-    if (v_cache.shape[:3] != k_cache.shape[:3] or k_scale_cache.shape != k_cache.shape[:3] or
-            v_scale_cache.shape != k_cache.shape[:3] or
-            (k_cache.shape[3] if k_cache.dtype == torch.int8 else k_cache.shape[3] // 8 * 16) != hs):
+    k_shape, v_shape = k_cache.shape, v_cache.shape
+    places, seqs, nkv = k_shape[:3], seqused_k.shape[0], k_shape[2]
+    hs = v_shape[3] // 8 * 16  # (an int4 half's view may have its word's 4 bytes behind the codes)
+    if (v_shape[:3] != places or k_scale_cache.shape != places or v_scale_cache.shape != places or
+            (k_shape[3] if k_cache.dtype == torch.int8 else k_shape[3] // 8 * 16) != hs):
         raise ValueError("evict_keys: the four cache views do not belong together")
     if seqused_k.dtype != torch.int32 or seqused_k.dim() != 1 or not seqused_k.is_contiguous():
         raise ValueError("evict_keys: seqused_k must be a contiguous int32 vector")
@@ -65,20 +67,27 @@ def evict_keys(k_cache, v_cache, k_scale_cache, v_scale_cache, weights, *, sequs
     _rows("new_weights", new_weights, torch.float32, seqs, nkv, budget)
     if new_seqused_k.dtype != torch.int32 or new_seqused_k.shape != (seqs,) or not new_seqused_k.is_contiguous():
         raise ValueError(f"evict_keys: new_seqused_k must be {seqs} contiguous int32 entries")
-    if seqs and block_table.numel() and new_block_table.data_ptr() == block_table.data_ptr():
+    table_at, new_table_at, used_at, new_used_at = (block_table.data_ptr(), new_block_table.data_ptr(), seqused_k.data_ptr(),
+                                                    new_seqused_k.data_ptr())
+    weights_at, new_weights_at = weights.data_ptr(), new_weights.data_ptr()
+    if seqs and block_table.numel() and new_table_at == table_at:
         raise ValueError("evict_keys: the kept cells move to other blocks: new_block_table must not be block_table")
-    if seqs and (new_weights.data_ptr() == weights.data_ptr() or new_seqused_k.data_ptr() == seqused_k.data_ptr()):
+    if seqs and (new_weights_at == weights_at or new_used_at == used_at):
         raise ValueError("evict_keys: weights and seqused_k are read while the new ones are written: give other tensors")
-    _hip.same_device("evict_keys", k_cache, v_cache=v_cache, k_scale_cache=k_scale_cache, v_scale_cache=v_scale_cache,
-                     weights=weights, seqused_k=seqused_k, block_table=block_table, new_block_table=new_block_table,
-                     kept=kept, new_weights=new_weights, new_seqused_k=new_seqused_k)
+    index = k_cache.get_device()
+    if index < 0 or not (index == v_cache.get_device() == k_scale_cache.get_device() == v_scale_cache.get_device() ==
+                         weights.get_device() == seqused_k.get_device() == block_table.get_device() ==
+                         new_block_table.get_device() == kept.get_device() == new_weights.get_device() ==
+                         new_seqused_k.get_device()):
+        _hip.same_device("evict_keys", k_cache, v_cache=v_cache, k_scale_cache=k_scale_cache, v_scale_cache=v_scale_cache,
+                         weights=weights, seqused_k=seqused_k, block_table=block_table, new_block_table=new_block_table,
+                         kept=kept, new_weights=new_weights, new_seqused_k=new_seqused_k)
     cache = _hip.paged_cache(k_cache, v_cache, k_scale_cache, v_scale_cache, hs)
     ws, ks, ns = weights.stride(), kept.stride(), new_weights.stride()
     args = _hip.EvictArgs()
-    _PACK.pack(args, weights.data_ptr(), ws[0], ws[1], seqused_k.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-               new_block_table.data_ptr(), new_block_table.stride(0), block_table.shape[1], new_block_table.shape[1], seqs,
-               int(max_seqlen_k), budget, sinks, recent, kept.data_ptr(), ks[0], ks[1], new_weights.data_ptr(), ns[0],
-               ns[1], new_seqused_k.data_ptr(), 0, 0)
+    _PACK.pack(args, weights_at, ws[0], ws[1], used_at, table_at, block_table.stride(0), new_table_at,
+               new_block_table.stride(0), block_table.shape[1], new_block_table.shape[1], seqs, int(max_seqlen_k), budget,
+               sinks, recent, kept.data_ptr(), ks[0], ks[1], new_weights_at, ns[0], ns[1], new_used_at, 0, 0)
     lib = _hip.lib()
     with _hip.on_device_of(k_cache):
         need = lib.qp_evict_workspace_size(cache, args)

@@ -63,8 +63,13 @@ def key_weights(q, k_cache, k_scale_cache, out, *, cu_seqlens_q, seqused_k, bloc
         raise ValueError(f"key_weights: query_signs must be {hs} contiguous fp32 signs")
     if torch.is_grad_enabled() and q.requires_grad:
         raise NotImplementedError("key_weights: no backward pass; call it under torch.no_grad()")
-    _hip.same_device("key_weights", q, k_cache=k_cache, k_scale_cache=k_scale_cache, out=out, cu_seqlens_q=cu_seqlens_q,
-                     seqused_k=seqused_k, block_table=block_table, query_signs=query_signs, previous=previous)
+    index = q.get_device()
+    if (index < 0 or not (index == k_cache.get_device() == k_scale_cache.get_device() == out.get_device() ==
+                          cu_seqlens_q.get_device() == seqused_k.get_device() == block_table.get_device()) or
+            (query_signs is not None and query_signs.get_device() != index) or
+            (previous is not None and previous.get_device() != index)):
+        _hip.same_device("key_weights", q, k_cache=k_cache, k_scale_cache=k_scale_cache, out=out, cu_seqlens_q=cu_seqlens_q,
+                         seqused_k=seqused_k, block_table=block_table, query_signs=query_signs, previous=previous)
     if k_scale_cache.dtype not in _hip._WORD_DTYPES:
         raise ValueError(f"key_weights: scale words must be 4-byte elements, got {k_scale_cache.dtype}")
     cs, ws, qs, os = k_cache.stride(), k_scale_cache.stride(), q.stride(), out.stride()

@@ -36,7 +36,10 @@ def _check(q, k, v, out, cu_q, cu_k, lse):
         raise ValueError(f"prompt_attention: lse must be fp32 {tuple(q.shape[:2])}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise NotImplementedError("prompt_attention: no backward pass; call it under torch.no_grad()")
-    _hip.same_device("prompt_attention", q, k=k, v=v, out=out, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, lse=lse)
+    index = q.get_device()
+    if not (index == k.get_device() == v.get_device() == out.get_device() == cu_q.get_device() == cu_k.get_device()) or \
+            index < 0 or (lse is not None and lse.get_device() != index):
+        _hip.same_device("prompt_attention", q, k=k, v=v, out=out, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, lse=lse)
 
 
 def prompt_attention(q, k, v, out=None, *, cu_seqlens_q, cu_seqlens_k=None, max_seqlen_k=None, max_seqlen_q=None,
