@@ -44,6 +44,37 @@ def test_prompt_of_many_rows(device, dtype, causal):
     run_prompt(device, lens, 32, 8, 128, {"bf16": torch.bfloat16, "fp16": torch.float16}[dtype], causal=causal, seed=2)
 
 
+@pytest.mark.parametrize("hs,nq,nkv", [(64, 16, 16), (128, 32, 16), (256, 16, 16), (512, 16, 8)])
+def test_prompts_by_length(device, hs, nq, nkv):
+    """Few sequences of many row blocks: earlier keys, none, fewer keys than queries, no queries, equal lengths. The longest
+    context's bound only decides the order of the blocks, whatever it says."""
+    import torch
+
+    from vllm_quantpack.attention.prompt import prompt_attention
+    lens = [(300, 300), (0, 70), (257, 900), (400, 130), (1, 512), (300, 300), (420, 421)]
+    run_prompt(device, lens, nq, nkv, hs, torch.bfloat16, num_splits=1, seed=hs, extra=2)
+    T, K = sum(t for t, _ in lens), sum(n for _, n in lens)
+    g = torch.Generator(device=device).manual_seed(3)
+    q = torch.randn((T, nq, hs), generator=g, device=device).to(torch.float16)
+    k, v = (torch.randn((K, nkv, hs), generator=g, device=device).to(torch.float16) for _ in range(2))
+    offsets = [i32(np.concatenate(([0], np.cumsum([x[i] for x in lens]))), device) for i in range(2)]
+
+    def call(bound):
+        return prompt_attention(q, k, v, cu_seqlens_q=offsets[0], cu_seqlens_k=offsets[1], max_seqlen_k=bound, num_splits=1)
+
+    want = torch.cat([prompt_attention(q[a:b], k[c:d], v[c:d], cu_seqlens_q=i32([0, b - a], device),
+                                       cu_seqlens_k=i32([0, d - c], device), num_splits=1)
+                      for a, b, c, d in zip(offsets[0][:-1].tolist(), offsets[0][1:].tolist(), offsets[1][:-1].tolist(),
+                                            offsets[1][1:].tolist()) if b > a])
+    for bound in (0, 1, 64, 900, K):
+        got = call(bound)
+        assert bool(torch.isfinite(got.float()).all())
+        # (a sequence for itself may have its rows in other blocks, whose running maxima differ: two results, each off by u of
+        # itself and u of the mean |v|, u = 2^-11, and by far less for its fp32 part)
+        assert torch.allclose(got.float(), want.float(), rtol=2 ** -10, atol=2 ** -10 * float(v.abs().max())), bound
+        assert torch.equal(got, call(900)), bound
+
+
 @pytest.mark.parametrize("hs,num_splits", [(128, 0), (512, 0), (64, 1)])
 def test_prompt_offsets_past_32_bits(device, hs, num_splits):
     """Key and value rows 64 Ki elements apart: the last ones lie 2^32 elements from the first."""
