@@ -75,6 +75,40 @@ def test_prompts_by_length(device, hs, nq, nkv):
         assert torch.equal(got, call(900)), bound
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_of_halved_keys(device, causal, hs, dtype):
+    """As many row blocks as CUs over long contexts, whose keys are halved between a workgroup's waves; contexts of one tile,
+    and of none, among them."""
+    import torch
+    lens = [(300, 1300), (1, 1100), (257, 257), (0, 40), (40, 64), (60, 65), (130, 100), (2, 0)]
+    run_prompt(device, lens, 48, 24, hs, {"bf16": torch.bfloat16, "fp16": torch.float16}[dtype], causal=causal, seed=hs)
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("at", [20, 600, 700, 1290])
+def test_prompt_infinities_in_halved_keys(device, hs, at):
+    """An infinite value reaches the rows that see its key and no others."""
+    import torch
+
+    from vllm_quantpack.attention.prompt import prompt_attention
+    g = torch.Generator(device=device).manual_seed(at)
+    T, K = 700, 1300
+    q = torch.randn((T, 48, hs), generator=g, device=device).to(torch.bfloat16)
+    k, v = (torch.randn((K, 24, hs), generator=g, device=device).to(torch.bfloat16) for _ in range(2))
+    v[at, :, 3] = 0.0
+    offsets = dict(cu_seqlens_q=i32([0, T], device), cu_seqlens_k=i32([0, K], device))
+    want = prompt_attention(q, k, v, **offsets)
+    v[at, :, 3] = float("inf")
+    got = prompt_attention(q, k, v, **offsets)
+    see = torch.arange(T, device=device) + K - T >= at
+    assert bool((got[see][..., 3] == float("inf")).all())
+    assert torch.equal(got[~see], want[~see])
+    rest = [c for c in range(hs) if c != 3]
+    assert torch.equal(got[..., rest], want[..., rest])
+
+
 @pytest.mark.parametrize("hs,num_splits", [(128, 0), (512, 0), (64, 1)])
 def test_prompt_offsets_past_32_bits(device, hs, num_splits):
     """Key and value rows 64 Ki elements apart: the last ones lie 2^32 elements from the first."""

@@ -34,9 +34,19 @@ struct PromptParams {
   int64_t ls0, ls1;
   float *so, *smax, *ssum;  // split partials: [token, head, split, HS], [token, head, split]
   int32_t num_seqs, num_tokens, num_keys, num_q_heads, num_kv_heads, num_splits, min_keys, causal;
+  int32_t group_keys;  // the longest context, where a block's keys may be halved between groups of waves (else 0)
   int32_t step;  // the row blocks of all sequences are taken in the order of their keys, in steps of so many (0: they are not)
   float scale_log2;
 };
+
+// The arguments, loaded where this is called: what only a kernel's end needs would take scalar registers all the way to it.
+__device__ __forceinline__ PromptParams late_params() {
+  auto at = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  PromptParams p;
+  __builtin_memcpy(&p, (const void *)at, sizeof p);
+  return p;
+}
 
 constexpr float kPromptNone = -1e30f;  // a row's maximum before it has seen a key
 // A row's maximum m is raised when a score exceeds it by more than this (log2 units): probabilities stay below 2^8, well
@@ -322,14 +332,17 @@ __device__ __forceinline__ void store_row(const PromptParams &p, const PromptBlo
 
 // ------------------------------------------------------------------------------------- heads of 64, 128 and 256
 
-template <int HS_, bool F16_, int WAVES>
+template <int HS_, bool F16_, int WAVES, int GROUPS = 1>
 struct PromptShape {
   static constexpr int HS = HS_;
   static constexpr bool F16 = F16_;
   // Two waves per SIMD up to head 128, in one workgroup or two: prompt_rows says which. At 256 a wave takes 512 registers.
   static constexpr int kWaves = WAVES;
   static constexpr int kWavesPerSimd = HS <= 128 ? 2 : 1;
-  static constexpr int kThreads = kWaves * 64;
+  // Two groups of waves share the rows, each with half of the keys, tiles of its own and a share of the sums, which are
+  // joined through LDS at the end: twice the waves where there are few blocks.
+  static constexpr int kGroups = GROUPS;
+  static constexpr int kThreads = kGroups * kWaves * 64;
   static constexpr int kRows = kWaves * 32;
   static constexpr int kKeys = 64;                   // keys per tile, two sub-tiles of 32
   static constexpr int kU = HS / 8;                  // 16-byte units of a row
@@ -340,7 +353,7 @@ struct PromptShape {
   static constexpr int kCopies = kTile / 1024 / kWaves;  // 1 KiB copies of a wave, K and V each
   static constexpr int kCopyRows = kWaves * 64 / kU;     // rows of copy i of all waves
   static constexpr int kOffsets = kCopyRows >= 16 ? 1 : kCopies;
-  static_assert(kTile % (1024 * kWaves) == 0 && kLds <= 160 * 1024, "LDS");
+  static_assert(kTile % (1024 * kWaves) == 0 && kGroups * kLds <= 160 * 1024, "LDS");
   // Position of unit c in row r of a K tile: 16 rows' reads of one unit hit every bank of the LDS once.
   static __host__ __device__ constexpr int k_swz(int r, int c) { return HS == 64 ? c ^ ((r >> 1) & 7) : c ^ (r & 15); }
   // The same in a V tile, in blocks of four units (32 channels, what a transposing read takes of a row): the four rows of
@@ -355,13 +368,16 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
   constexpr int HS = Sh::HS, KT = Sh::kKeys, U = Sh::kU;
   constexpr bool F16 = Sh::F16;
   constexpr int kCs = HS / 16, kCt = HS / 32;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[Sh::kLds];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[Sh::kGroups * Sh::kLds];
   PromptBlock b;
   if (!prompt_block<Sh::kRows>(p, b)) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w = wave % Sh::kWaves, group = wave / Sh::kWaves;
+  const int place = group * Sh::kLds;  // of the group's tiles
   const int col = lane & 31, h = lane >> 5;
   const int G = p.num_q_heads / p.num_kv_heads;
-  const int kb = b.kb, ke = b.ke;
+  // the group's keys [kb, ke), of which there may be none in the last one; every wave walks ntiles tiles
+  const int tiles = b.ke > b.kb ? (b.ke - b.kb + KT - 1) / KT : 0, ntiles = (tiles + Sh::kGroups - 1) / Sh::kGroups;
+  const int kb = b.kb + group * ntiles * KT, ke = group == Sh::kGroups - 1 ? b.ke : min(b.ke, kb + ntiles * KT);
   auto last_pos = [&](int row) { return p.causal ? b.n - b.qlen + row / G : b.n - 1; };  // the last key that a row sees
 
   // ---- the wave's rows: lane row col -> (token rr / G, query head rr % G)
@@ -381,7 +397,6 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
 #pragma unroll
   for (int ct = 0; ct < kCt; ++ct) acc[ct] = f32x16_t{};
 
-  const int ntiles = ke > kb ? (ke - kb + KT - 1) / KT : 0;
   if (ntiles > 0) {
     auto seen = [&](int row) { return max(0, min(last_pos(row) + 1, ke) - kb); };  // keys of the split that a row sees
     const int wplain = uniform(active ? seen(wrow) : 0) / 32;  // sub-tiles that every row of the wave sees whole,
@@ -389,7 +404,7 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
 
     // ---- HBM -> LDS: copy i of a wave fills 16-byte units 64 (w + kWaves i) .. of the tile, lane by lane; the unit's row
     // and column are those that the swizzle puts there
-    const uint32_t lds0 = lds_addr(smem);
+    const uint32_t lds0 = lds_addr(smem) + place;
     const uint8_t *kbase = reinterpret_cast<const uint8_t *>(p.k + (int64_t)(b.k0 + kb) * p.ks0 + (int64_t)b.kvh * p.ks1);
     const uint8_t *vbase = reinterpret_cast<const uint8_t *>(p.v + (int64_t)(b.k0 + kb) * p.vs0 + (int64_t)b.kvh * p.vs1);
     const uint32_t ksb = (uint32_t)(p.ks0 * 2), vsb = (uint32_t)(p.vs0 * 2);
@@ -403,6 +418,7 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
     }
     auto copy = [&](int t, int kslot, int vslot) {
       const int left = ke - kb - t * KT - 1;  // the tile's last key (rows past it repeat it: always mapped memory)
+      if (Sh::kGroups > 1 && left < 0) return;
       const uint8_t *kt = kbase + (int64_t)t * KT * ksb, *vt = vbase + (int64_t)t * KT * vsb;
 #pragma unroll
       for (int i = 0; i < Sh::kCopies; ++i) {
@@ -411,11 +427,11 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
         const uint8_t *kc = kt + (int64_t)base * ksb, *vc = vt + (int64_t)base * vsb;
         uint32_t ko = kvo[i % Sh::kOffsets], vo = vvo[i % Sh::kOffsets];
         if (left < KT - 1) {
+          const int over = max(0, (64 * (w + Sh::kWaves * (i % Sh::kOffsets)) + lane) / U + base - left);
           kc = kt;
           vc = vt;
-          const int d = at + lane, r = d / U, c = d % U, rs = min(r, left);
-          ko = (uint32_t)rs * ksb + 16u * (uint32_t)Sh::k_swz(r, c);
-          vo = (uint32_t)rs * vsb + 16u * (uint32_t)Sh::v_swz(r, c);
+          ko += (uint32_t)(base - over) * ksb;
+          vo += (uint32_t)(base - over) * vsb;
         }
         dma16_saddr<false>(kc, ko, lds0 + (uint32_t)(kslot * Sh::kTile + 16 * at));
         dma16_saddr<false>(vc, vo, lds0 + (uint32_t)(Sh::kOffV + vslot * Sh::kTile + 16 * at));
@@ -426,10 +442,10 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
     constexpr int kKo = kCs < 8 ? kCs : 8, kVo = kCt < 4 ? kCt : 4;
     uint32_t koff[kKo], voff[kVo];
 #pragma unroll
-    for (int i = 0; i < kKo; ++i) koff[i] = col * (2 * HS) + 16 * Sh::k_swz(col, 2 * i + h);
+    for (int i = 0; i < kKo; ++i) koff[i] = place + col * (2 * HS) + 16 * Sh::k_swz(col, 2 * i + h);
 #pragma unroll
     for (int i = 0; i < kVo; ++i)
-      voff[i] = v_row(lane) * (2 * HS) + 16 * Sh::v_swz(v_row(lane), 4 * i) + 2 * v_channel(lane);
+      voff[i] = place + v_row(lane) * (2 * HS) + 16 * Sh::v_swz(v_row(lane), 4 * i) + 2 * v_channel(lane);
     auto k_op = [&](const uint8_t *kt, int cs) {
       return *reinterpret_cast<const u32x4_t *>(kt + koff[cs % kKo] + 256 * (cs / kKo));
     };
@@ -499,7 +515,7 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
     using No = std::false_type;
     using Yes = std::true_type;
     copy(0, 0, 0);
-    if (ntiles > 1) {
+    if (ke - kb > KT) {
       copy(1, 1, 1);
       wait_vmcnt<2 * Sh::kCopies>();
     } else {
@@ -535,7 +551,7 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
         const int g = 2 * t + u;
         if (g >= wend) continue;
         const uint8_t *kn = u == 0 ? k_at(t) + 64 * HS : k_at(t + 1), *vt = tile + u * 64 * HS;
-        if (g >= wplain && odd_values<HS, F16>(vt, lane)) {
+        if (g >= wplain && odd_values<HS, F16>(vt + place, lane)) {
           body(kn, vt, g, Yes{}, Yes{});
           Odd<F16>::restore(acc, vbase + (int64_t)(32 * g) * vsb + 32 * h, vsb, kb + 32 * g, min(ke, kb + 32 * g + 32), row_pos);
         } else {
@@ -545,7 +561,39 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
       vslot = vslot == 2 ? 0 : vslot + 1;
     }
   }
-  store_row<HS, F16>(p, b, tok, jh, 16 * h, h == 0, m, l + shfl_xor_f(l, 32), acc);
+  if constexpr (Sh::kGroups > 1) {
+    if (ntiles > 0) {
+      constexpr int kWave = kCt * 4096 + 512;  // a wave's sums, then its statistics
+      f32x4_t *sums = reinterpret_cast<f32x4_t *>(smem + w * kWave) + lane;
+      float2 *stats = reinterpret_cast<float2 *>(smem + w * kWave + kCt * 4096) + lane;
+      __syncthreads();
+      if (group == 1) {
+#pragma unroll
+        for (int ct = 0; ct < kCt; ++ct)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sums[64 * (4 * ct + i)] = f32x4_t{acc[ct][4 * i], acc[ct][4 * i + 1], acc[ct][4 * i + 2], acc[ct][4 * i + 3]};
+        *stats = make_float2(m, l);
+      }
+      __syncthreads();
+      if (group == 1) return;
+      const float2 st = *stats;
+      const float to = fmaxf(m, st.x), own = __builtin_amdgcn_exp2f(m - to), other = __builtin_amdgcn_exp2f(st.x - to);
+      m = to;
+      l = l * own + st.y * other;
+#pragma unroll
+      for (int ct = 0; ct < kCt; ++ct)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4_t x = sums[64 * (4 * ct + i)];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[ct][4 * i + j] = acc[ct][4 * i + j] * own + x[j] * other;
+        }
+    } else if (group == 1) {
+      return;
+    }
+  }
+  store_row<HS, F16>(late_params(), b, tok, jh, 16 * h, h == 0, m, l + shfl_xor_f(l, 32), acc);
 }
 
 // -------------------------------------------------------------------------------------------- heads of 512
@@ -672,7 +720,7 @@ __global__ __launch_bounds__(256) void prompt_wide_kernel(const PromptParams p) 
                           min(ke, kb + (t + 1) * KT), row_pos);
     }
   }
-  store_row<HS, F16>(p, b, tok, jh, kHc * part + 16 * h, h == 0 && part == 0, m, l + shfl_xor_f(l, 32), acc);
+  store_row<HS, F16>(late_params(), b, tok, jh, kHc * part + 16 * h, h == 0 && part == 0, m, l + shfl_xor_f(l, 32), acc);
 }
 
 // The log-sum-exp merge of split partials, kPer waves per (token, query head) row: the row's splits weighed by
@@ -801,15 +849,26 @@ int64_t prompt_partial_bytes(const qp_prompt_args *a, int splits) {
   return (int64_t)a->num_tokens * a->num_q_heads * splits * (a->head_size + 2) * 4;
 }
 
+// Groups of waves that share a block's keys: two where there are up to three blocks for two CUs and 1024 keys or more, us with
+// two and with one, 32 / 8 heads of 128 and of 64: 1000 tokens after 8000 155 / 169, 96 / 112, after 2048 58 / 63, 37 / 43; four
+// turns of up to 509 tokens over up to 4605 keys 65 / 73, 46 / 50; 600 tokens 20 / 19; 2048 tokens, two blocks per CU, 54 / 54,
+// 36 / 33.
+int prompt_groups(const PromptParams &p, dim3 grid) {
+  return p.group_keys >= 1024 && 2 * (int64_t)grid.x * grid.y <= 3 * (int64_t)device_cus() ? 2 : 1;
+}
+
 template <int HS, bool F16>
 void launch_prompt(const PromptParams &p, int rows, dim3 grid, hipStream_t s) {
   const uint32_t share = prompt_share(grid.y * grid.z);
   grid.x = ((grid.x + (1u << share) - 1) >> share) << share;
   if constexpr (HS == 512) {
     prompt_wide_kernel<F16><<<grid, 256, 0, s>>>(p);
-  } else if constexpr (HS == 128) {
-    if (rows == 256) prompt_kernel<PromptShape<HS, F16, 8>><<<grid, 512, 0, s>>>(p);
-    else prompt_kernel<PromptShape<HS, F16, 4>><<<grid, 256, 0, s>>>(p);
+  } else if constexpr (HS == 256) {
+    prompt_kernel<PromptShape<HS, F16, 4>><<<grid, 256, 0, s>>>(p);
+  } else if (HS == 128 && rows == 256) {
+    if constexpr (HS == 128) prompt_kernel<PromptShape<HS, F16, 8>><<<grid, 512, 0, s>>>(p);
+  } else if (prompt_groups(p, grid) == 2) {
+    prompt_kernel<PromptShape<HS, F16, 4, 2>><<<grid, 512, 0, s>>>(p);
   } else {
     prompt_kernel<PromptShape<HS, F16, 4>><<<grid, 256, 0, s>>>(p);
   }
@@ -904,6 +963,7 @@ extern "C" int qp_prompt(const qp_prompt_args *a, qp_stream_t stream) {
   p.num_splits = splits;
   p.min_keys = a->num_splits == 0 ? kPromptSplitKeys : 0;
   p.causal = a->causal != 0;
+  p.group_keys = a->num_splits == 0 && splits == 1 ? a->max_seqlen_k : 0;
   // A few sequences whose blocks take turns: longest first, which costs a workgroup 0.1 us and as much for every two sequences.
   // In order of length against order of place, us: four turns of up to 509 tokens over up to 4605 keys, 32 / 8 heads of 64,
   // 48 / 61, of 128 72 / 88; prompts of up to 2048 tokens, heads of 128, 3 of them 67 / 71, 8 152 / 154 and 85 / 86; 12 of up
