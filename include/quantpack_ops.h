@@ -41,8 +41,8 @@ typedef struct qp_prompt_args {
   int32_t num_kv_heads;
   int32_t head_size;           /* 64, 128, 256 or 512 */
   int32_t dtype;               /* QP_DTYPE_BF16 or QP_DTYPE_F16: query, key, value and out */
-  int32_t max_seqlen_k;        /* longest sequence's keys: bounds the automatic split count */
-  int32_t num_splits;          /* key splits per row block, at most 128; 0 = automatic */
+  int32_t max_seqlen_k;        /* longest sequence's keys: what the work is laid out by, with any value correct */
+  int32_t num_splits;          /* key splits per row block, at most 128; 1 = one walk over the keys; 0 = automatic */
   int32_t causal;
   float softmax_scale;         /* positive */
   void *out;                   /* [num_tokens, num_q_heads, head_size] */

@@ -1,4 +1,4 @@
-"""Build libquantpack_hip.so for gfx950 from csrc/*.hip with hipcc (objects in _build/, the library in-tree next to
+"""Build libquantpack_hip.so for gfx950 from csrc/*.hip and csrc/ops/*.hip with hipcc (objects in _build/, the library in-tree next to
 the Python package so that it travels with the source tree).
 
     python vllm-quantpack_amd/build.py [--jobs N] [--verbose] [--only a.hip,b.hip]
@@ -33,7 +33,7 @@ def hipcc():
 
 
 # Per-source extra flags. The prefill kernel keeps its QK^T MFMA results in VGPRs (its PV accumulators own the AGPRs);
-# the dual prefill kernel keeps all of them there (256 VGPRs per wave, no AGPRs).
+# the dual prefill kernel and those of csrc/ops keep all of them there (256 VGPRs per wave, no AGPRs).
 # The decode kernels take no NaN inputs (masked scores are -inf, never NaN), so their maxima need no quieting.
 EXTRA = {"qp_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "qp_prefill_dual.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
@@ -348,10 +348,10 @@ def _check_mfma(src, verbose, scheduled=False):
 
 
 def build(jobs=None, verbose=False, only=None):
-    """Compile every csrc/*.hip (or only the named ones, reusing the other objects of an earlier build), check the
+    """Compile every csrc/*.hip and csrc/ops/*.hip (or only the named ones, reusing the other objects of an earlier build), check the
     code of their MFMA loops and link the shared library. Returns the library path."""
     os.makedirs(OBJ, exist_ok=True)
-    srcs = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
+    srcs = sorted(os.path.join(d, f) for d in (CSRC, os.path.join(CSRC, "ops")) for f in os.listdir(d) if f.endswith(".hip"))
     todo = [s for s in srcs if not only or os.path.basename(s) in only]
     jobs = jobs or min(8, os.cpu_count() or 1, len(srcs))
     with cf.ThreadPoolExecutor(jobs) as ex:

@@ -2,8 +2,9 @@
 re-implemented as hand-written gfx950 HIP kernels behind the plugin's attention-backend API.
 
 Layout:
-  attention/  the drop-in Python boundary (int4_kv, int4_prefill, k8v4_kv, rht) over the HIP library
-  _hip.py     ctypes binding of libquantpack_hip.so (C ABI: include/quantpack.h)
+  attention/  the drop-in Python boundary (int4_kv, int4_prefill, k8v4_kv, rht) over the HIP library, and what stands
+              around the cache: prompt (attention over a prompt's own keys), key_weights and eviction
+  _hip.py     ctypes binding of libquantpack_hip.so (C ABI: include/quantpack.h, include/quantpack_ops.h)
   tools/      synthetic paged caches for the benchmark and the parity tests
 
 Only the KV-attention part of the reference plugin is here; its EXL3 quantisation, model families and TurboQuant

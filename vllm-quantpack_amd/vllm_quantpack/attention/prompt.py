@@ -54,9 +54,9 @@ def prompt_attention(q, k, v, out=None, *, cu_seqlens_q, cu_seqlens_k=None, max_
     written. Keys and values that no query sees are never used, whatever they hold.
 
     Strides are free as long as channels are contiguous and rows 16-byte aligned, so q, k and v may be views of one
-    projection's output. max_seqlen_k bounds the automatic key splits (num_splits 0) of batches with few rows, K when None;
-    max_seqlen_q is accepted for symmetry and not used. The partials of a split come from torch's caching allocator; no
-    host synchronisation."""
+    projection's output. max_seqlen_k, the longest sequence's keys (K when None), is what the work is laid out by: the
+    automatic key splits (num_splits 0) of batches with few rows, and the order of the row blocks. max_seqlen_q is accepted
+    for symmetry and not used. The partials of a split come from torch's caching allocator; no host synchronisation."""
     del max_seqlen_q
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
