@@ -1,5 +1,5 @@
-"""Build libquantpack_hip.so for gfx950 from csrc/*.hip and csrc/ops/*.hip with hipcc (objects in _build/, the library in-tree next to
-the Python package so that it travels with the source tree).
+"""Build libquantpack_hip.so for gfx950 from csrc/*.hip and csrc/ops/*.hip with hipcc (objects in _build/, the library
+in-tree next to the Python package so that it travels with the source tree).
 
     python vllm-quantpack_amd/build.py [--jobs N] [--verbose] [--only a.hip,b.hip]
 
@@ -348,8 +348,8 @@ def _check_mfma(src, verbose, scheduled=False):
 
 
 def build(jobs=None, verbose=False, only=None):
-    """Compile every csrc/*.hip and csrc/ops/*.hip (or only the named ones, reusing the other objects of an earlier build), check the
-    code of their MFMA loops and link the shared library. Returns the library path."""
+    """Compile every csrc/*.hip and csrc/ops/*.hip (or only the named ones, reusing the other objects of an earlier
+    build), check the code of their MFMA loops and link the shared library. Returns the library path."""
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(os.path.join(d, f) for d in (CSRC, os.path.join(CSRC, "ops")) for f in os.listdir(d) if f.endswith(".hip"))
     todo = [s for s in srcs if not only or os.path.basename(s) in only]

@@ -9,9 +9,10 @@
 // positions are too much for one workgroup per head: there the first histogram is made by many, which then put the weights of
 // the bin that the threshold lies in, a few per cent, into lists, and only those are looked at by the one.
 //
-// What bounds it, measured: 16384 of 131072 positions of 4 heads of 256 (int4) take 5.3 us for the histogram, 9 for the lists, 8.8
-// for the threshold, 15 for the cells (35 MB at 2.3 TB/s): four launches, each a chain of few dependent loads. With more to move the
-// cells' share grows: 16 contexts of up to 16384, 2048 kept, 8 heads of 128, int8 keys: 36 of 60 us, at 2.9 TB/s.
+// What bounds it, measured: 16384 of 131072 positions of 4 heads of 256 (int4) take 5.3 us for the histogram, 9 for the
+// lists, 8.8 for the threshold, 15 for the cells (35 MB at 2.3 TB/s): four launches, each a chain of few dependent loads.
+// With more to move the cells' share grows: 16 contexts of up to 16384, 2048 kept, 8 heads of 128, int8 keys: 36 of 60 us, at
+// 2.9 TB/s.
 #include "qp_common.h"
 #include "quantpack_ops.h"
 

@@ -8,10 +8,10 @@
 // Every weight has one owner, so no order of additions varies. With few query rows (a decode step) the scores are made once
 // and kept between the passes; with many (the last tokens of a prompt) they are made twice, from keys unpacked in registers.
 //
-// What bounds it, measured: one token, 24 / 4 heads of 256, over 131072 int4 keys takes 31 us for the scores and 9.5 for the sums.
-// A cell's key half lies beside its value half, so that nearly all lines of the cache are fetched: 138 MB for 66 of key codes, at
-// 4.45 TB/s. 64 tokens over 32768 keys, 64 / 8 heads of 128: 62 us for the statistics and 50 for the weights, 550 and 690 TFLOP/s,
-// exponentials and products taking about as long, and 10 for rows and statistics.
+// What bounds it, measured: one token, 24 / 4 heads of 256, over 131072 int4 keys takes 31 us for the scores and 9.5 for the
+// sums. A cell's key half lies beside its value half, so that nearly all lines of the cache are fetched: 138 MB for 66 of key
+// codes, at 4.45 TB/s. 64 tokens over 32768 keys, 64 / 8 heads of 128: 62 us for the statistics and 50 for the weights, 550
+// and 690 TFLOP/s, exponentials and products taking about as long, and 10 for rows and statistics.
 //
 // Precision: codes enter the product as code - 8 (int4) or as they are (int8), exact in bf16 and centred, so that the zero
 // point's share, sum(q) (zp - 8), takes away little; scores meet the row's maximum in one fused multiply-add.
@@ -668,9 +668,9 @@ KwPlan kw_plan(const qp_key_weights_args *a) {
   k.max_rows = (int64_t)a->max_query_len * (a->num_q_heads / a->num_kv_heads);
   k.score_stride = (keys + 3) / 4 * 4;
   const int64_t score_bytes = heads * k.max_rows * k.score_stride * 4;
-  // Few rows: their scores are kept (in up to 1 GiB) between the passes, instead of made twice. Kept against made twice, us, one
-  // sequence of 65536 int4 keys: heads of 64 (32 / 8), 16 rows 33 / 38, 32 rows 53 / 39; 128 (32 / 8), 16 rows 38 / 47, 32 rows
-  // 66 / 47; 256 (24 / 4), 24 rows 43 / 44; 512 (16 / 2), 16 rows 33 / 42, 32 rows 48 / 42.
+  // Few rows: their scores are kept (in up to 1 GiB) between the passes, instead of made twice. Kept against made twice, us,
+  // one sequence of 65536 int4 keys: heads of 64 (32 / 8), 16 rows 33 / 38, 32 rows 53 / 39; 128 (32 / 8), 16 rows 38 / 47,
+  // 32 rows 66 / 47; 256 (24 / 4), 24 rows 43 / 44; 512 (16 / 2), 16 rows 33 / 42, 32 rows 48 / 42.
   k.few = k.max_rows > 0 && k.max_rows <= 16 + std::min(a->head_size, 256) / 32 && score_bytes <= (int64_t(1) << 30);
   if (k.few) {
     k.subs = kKwSubs;  // long segments, unless they are too few to fill the GPU

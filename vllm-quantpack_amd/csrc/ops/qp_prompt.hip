@@ -12,10 +12,11 @@
 // and the packed probabilities are the B operand of the second product as they are. K and V tiles are copied to LDS as they
 // lie in memory, a tile ahead of their use; the V^T operand comes from the LDS's transposing reads (ds_read_b64_tr_b16).
 //
-// What bounds it, measured: 16384 tokens, 32 / 8 heads of 128, take 1.97 ms = 1110 TFLOP/s. MFMAs keep the matrix pipes busy for
-// 56 % of the cycles at 1.9 GHz and the softmax the vector pipes for 53 %; the same kernel's MFMAs alone take 1.61 ms, without the
-// exponentials it takes 1.87, without the reads of K and V from LDS 1.84. A token over 65536 keys, 64 / 8 heads: 57 us for the walk =
-// 4.7 TB/s, and 4.7 for the merge. Small batches are bound by the blocks with the most keys and by each block's start, 3 to 4 us.
+// What bounds it, measured: 16384 tokens, 32 / 8 heads of 128, take 1.97 ms = 1110 TFLOP/s. MFMAs keep the matrix pipes busy
+// for 56 % of the cycles at 1.9 GHz and the softmax the vector pipes for 53 %; the same kernel's MFMAs alone take 1.61 ms,
+// without the exponentials it takes 1.87, without the reads of K and V from LDS 1.84. A token over 65536 keys, 64 / 8 heads:
+// 57 us for the walk = 4.7 TB/s, and 4.7 for the merge. Small batches are bound by the blocks with the most keys and by each
+// block's start, 3 to 4 us.
 #include "qp_common.h"
 #include "quantpack_ops.h"
 
@@ -44,7 +45,8 @@ struct PromptParams {
   float scale_log2;
 };
 
-// The arguments, loaded where this is called: what only a kernel's end needs would take scalar registers all the way to it.
+// The kernels' one argument, loaded where this is called: what only a kernel's end needs would take scalar registers all the
+// way to it.
 __device__ __forceinline__ PromptParams late_params() {
   auto at = __builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(at));
@@ -830,11 +832,11 @@ int64_t prompt_blocks(const qp_prompt_args *a) {
   return (int64_t)a->num_tokens * (a->num_q_heads / a->num_kv_heads) / prompt_rows(a) + a->num_seqs;
 }
 
-// Key splits of a call, of 256 keys at least: 1 where the row blocks alone fill the GPU, else the count with the least estimate,
-// in tiles: rounds of workgroups by a split's tiles and the 6 that a workgroup's start and end cost, and the merge with its
-// launch and traffic. Measured, us, with one split and the count chosen: a token over 65536 keys, 64 / 8 heads of 128, 895 and
-// 52; twice 300 tokens over 9300, 32 / 8 heads, 166 and 119 (3 splits); 2048 tokens alone 53, but 107 with 2 splits: partials are
-// fp32 and pass through memory.
+// Key splits of a call, of 256 keys at least: 1 where the row blocks alone fill the GPU, else the count with the least
+// estimate, in tiles: rounds of workgroups by a split's tiles and the 6 that a workgroup's start and end cost, and the merge
+// with its launch and traffic. Measured, us, with one split and the count chosen: a token over 65536 keys, 64 / 8 heads of
+// 128, 895 and 52; twice 300 tokens over 9300, 32 / 8 heads, 166 and 119 (3 splits); 2048 tokens alone 53, but 107 with 2
+// splits: partials are fp32 and pass through memory.
 constexpr int kPromptSplitKeys = 256;
 
 int prompt_splits(const qp_prompt_args *a) {
@@ -859,10 +861,10 @@ int64_t prompt_partial_bytes(const qp_prompt_args *a, int splits) {
   return (int64_t)a->num_tokens * a->num_q_heads * splits * (a->head_size + 2) * 4;
 }
 
-// Groups of waves that share a block's keys: two where there are up to three blocks for two CUs and 1024 keys or more, us with
-// two and with one, 32 / 8 heads of 128 and of 64: 1000 tokens after 8000 155 / 169, 96 / 112, after 2048 58 / 63, 37 / 43; four
-// turns of up to 509 tokens over up to 4605 keys 65 / 73, 46 / 50; 600 tokens 20 / 19; 2048 tokens, two blocks per CU, 54 / 54,
-// 36 / 33.
+// Groups of waves that share a block's keys: two where there are up to three blocks for two CUs and 1024 keys or more, us
+// with two and with one, 32 / 8 heads of 128 and of 64: 1000 tokens after 8000 155 / 169, 96 / 112, after 2048 58 / 63, 37 /
+// 43; four turns of up to 509 tokens over up to 4605 keys 65 / 73, 46 / 50; 600 tokens 20 / 19; 2048 tokens, two blocks per
+// CU, 54 / 54, 36 / 33.
 int prompt_groups(const PromptParams &p, dim3 grid) {
   return p.group_keys >= 1024 && 2 * (int64_t)grid.x * grid.y <= 3 * (int64_t)device_cus() ? 2 : 1;
 }

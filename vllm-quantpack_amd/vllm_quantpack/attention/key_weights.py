@@ -29,8 +29,9 @@ def key_weights(q, k_cache, k_scale_cache, out, *, cu_seqlens_q, seqused_k, bloc
     q bf16 [T, NQ, hs] in the cache's domain, or unrotated with query_signs (`rht.signs`), which rotates each row as it
     loads; k_cache (blocks, bs, NKV, bytes) uint8 nibble pairs or int8 with its scale words k_scale_cache (the views of
     `k8v4_kv`; an int4 view's bytes past the codes are not read); out fp32 [sequences, NKV, L] with max_seqlen_k <= L (L
-    when None); previous: None, or weights of the same shape (out itself for an update in place). softmax_scale multiplies q.k in the cache's domain, as in `prefill_attention`. A sequence's
-    query tokens are the last of its positions and see the keys up to their own; at most max_seqlen_q of them are counted.
+    when None); previous: None, or weights of the same shape (out itself for an update in place). softmax_scale multiplies
+    q.k in the cache's domain, as in `prefill_attention`. A sequence's query tokens are the last of its positions and see
+    the keys up to their own; the first max_seqlen_q of them are counted.
 
     A token that sees no key adds nothing, a sequence without tokens keeps its decayed weights, and a key on a page outside
     the cache gets none. The workspace comes from torch's caching allocator; no host synchronisation."""
@@ -79,8 +80,9 @@ def key_weights(q, k_cache, k_scale_cache, out, *, cu_seqlens_q, seqused_k, bloc
                _hip.CODES_INT8 if k_cache.dtype == torch.int8 else _hip.CODES_INT4, k_cache.shape[0], k_cache.shape[1], nkv,
                hs, q.data_ptr(), qs[0], qs[1], cu_seqlens_q.data_ptr(), seqused_k.data_ptr(), block_table.data_ptr(),
                block_table.stride(0), block_table.shape[1], seqs, q.shape[0], q.shape[1],
-               int(min(max_seqlen_q, q.shape[0])), int(max_seqlen_k), float(softmax_scale), float(decay), 0 if query_signs is None else query_signs.data_ptr(),
-               0 if previous is None else previous.data_ptr(), ps[0], ps[1], out.data_ptr(), os[0], os[1], 0, 0)
+               int(min(max_seqlen_q, q.shape[0])), int(max_seqlen_k), float(softmax_scale), float(decay),
+               0 if query_signs is None else query_signs.data_ptr(), 0 if previous is None else previous.data_ptr(), ps[0],
+               ps[1], out.data_ptr(), os[0], os[1], 0, 0)
     lib = _hip.lib()
     with _hip.on_device_of(q):
         need = lib.qp_key_weights_workspace_size(args)
