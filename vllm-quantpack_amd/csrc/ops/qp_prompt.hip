@@ -55,9 +55,15 @@ __device__ __forceinline__ PromptParams late_params() {
   return p;
 }
 
-constexpr float kPromptNone = -1e30f;  // a row's maximum before it has seen a key
-// A row's maximum m is raised when a score exceeds it by more than this (log2 units): probabilities stay below 2^8, well
-// within fp16, whose smallest normal number is then 2^-22 of the largest probability.
+constexpr float kPromptNone = -1e30f;  // a row's reference before it has seen a key
+// A row's scores are taken relative to a reference m (log2 units), its running maximum less prompt_below. It is raised when a
+// score exceeds it by kPromptHeadroom more than that, so the largest probability lies between 2^below and 2^(below + headroom),
+// and the row's sum above 2^below. bf16 has the exponents of fp32. fp16 loses bits below 2^-14 and has nothing below 2^-25, while
+// the sum takes unrounded probabilities: with the largest at 2^7 or more, and at most 2^15, a key loses 2^-32 of the sum at
+// most. Relative to the maximum itself, 65536 keys 17 nats below another's came out 43 % wrong, and 18 nats below as nothing; a
+// call takes up to 1 % longer.
+template <bool F16>
+constexpr float prompt_below = F16 ? 7.f : 0.f;
 constexpr float kPromptHeadroom = 8.f;
 constexpr int kPromptWideRows = 64;       // rows of a workgroup at head 512
 
@@ -284,14 +290,18 @@ __device__ __forceinline__ void mask_scores(f32x16_t &x, int key0, int row_pos, 
   }
 }
 
-// A row's maximum m is raised to `top` (the largest score of the lane's keys) where that exceeds it by the headroom, and
-// what was summed up relative to the old one is scaled. A row's bits do not go by its neighbours': each is raised for itself.
-template <int CT>
+// A row's reference m is raised for `top` (the largest score of the lane's keys, unscaled) where that exceeds it by more than the
+// headroom, and what was summed up relative to the old one is scaled. A row's bits do not go by its neighbours': each is raised
+// for itself. In fp16 the difference is the one that the exponentials take, so that none exceeds the type's range, however large
+// the scores; bf16 has room for the scaled score's rounding (with fp16's form a token over 65536 keys takes 63.6 us, not 61.5).
+template <bool F16, int CT>
 __device__ __forceinline__ void raise(float top, float scale_log2, float &m, float &l, f32x16_t (&acc)[CT]) {
-  top *= scale_log2;
-  if (__any(top > m + kPromptHeadroom)) {
+  constexpr float kMost = prompt_below<F16> + kPromptHeadroom;
+  if (!F16) top *= scale_log2;
+  auto exceeds = [&](float x) { return F16 ? fmaf(x, scale_log2, -m) > kMost : x > m + kMost; };
+  if (__any(exceeds(top))) {
     const float most = other_half_max(top);
-    const float to = most > m + kPromptHeadroom ? most : m;
+    const float to = exceeds(most) ? (F16 ? fmaf(most, scale_log2, -prompt_below<F16>) : most) : m;
     const float alpha = __builtin_amdgcn_exp2f(m - to);
     m = to;
     l *= alpha;
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
         }
       }
       s = sn;
-      raise(top, p.scale_log2, m, l, acc);
+      raise<F16>(top, p.scale_log2, m, l, acc);
     };
 
     // ---- the walk. Tile t's last sub-tile is worked through beside the first scores of tile t + 1: before it the waves
@@ -534,7 +544,7 @@ __global__ __launch_bounds__(Sh::kThreads, Sh::kWavesPerSimd) void prompt_kernel
 #pragma unroll
       for (int c = 0; c < kCs; ++c) s = mfma_prompt<F16>(k_op(smem, c), qop[c], s);
       if (wplain == 0) mask_scores(s, kb + 4 * h, row_pos, ke);
-      raise(largest(s), p.scale_log2, m, l, acc);
+      raise<F16>(largest(s), p.scale_log2, m, l, acc);
     }
     int t = 0, vslot = 0;
     auto k_at = [&](int t) { return smem + (t & 1) * Sh::kTile; };
@@ -688,7 +698,7 @@ __global__ __launch_bounds__(256) void prompt_wide_kernel(const PromptParams p) 
         for (int j = 0; j < 4; ++j) s[4 * i + j] += x[j];
       }
       if constexpr (MASK) mask_scores(s, kb + t * KT + 4 * h, row_pos, ke);
-      raise(largest(s), p.scale_log2, m, l, acc);
+      raise<F16>(largest(s), p.scale_log2, m, l, acc);
       u32x4_t pop[2];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
