@@ -768,7 +768,7 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(const PromptParams p)
   k0 = max(0, k0);
   const int n = max(0, min(k1, p.num_keys) - k0);
   const int seg = segment_keys(n, p.num_splits, p.min_keys);
-  const int used = min(p.num_splits, (int)(((int64_t)n + seg - 1) / seg));
+  const int used = segments_used(n, p.num_splits, seg);
   const float *smax = p.smax + row * p.num_splits, *ssum = p.ssum + row * p.num_splits;
   const float m0 = lane < used ? smax[lane] : kPromptNone, m1 = lane + 64 < used ? smax[lane + 64] : kPromptNone;
   const float l0 = lane < used ? ssum[lane] : 0.f, l1 = lane + 64 < used ? ssum[lane + 64] : 0.f;

@@ -341,8 +341,17 @@ namespace qp {
 // Keys per segment of a context of n keys cut into at most `segments` of them: whole 32-key chunks, and no fewer than
 // min_keys (0: no such floor). The kernels that write partials and the merge that reads them use the same rule;
 // segments that start at or past the context have nothing.
-__device__ __forceinline__ int segment_keys(int n, int segments, int min_keys) {
-  return max((n + segments * QP_DECODE_TILE - 1) / (segments * QP_DECODE_TILE) * QP_DECODE_TILE, min_keys);
+__host__ __device__ __forceinline__ int segment_keys(int n, int segments, int min_keys) {
+  const int keys = (n + segments * QP_DECODE_TILE - 1) / (segments * QP_DECODE_TILE) * QP_DECODE_TILE;
+  return keys > min_keys ? keys : min_keys;
+}
+
+// The segments of `seg` keys (segment_keys) that a context of n keys has something in, the first ones. A context without keys
+// has none, and without a floor its segments have no length to divide by.
+__host__ __device__ __forceinline__ int segments_used(int n, int segments, int seg) {
+  if (n <= 0) return 0;
+  const int64_t used = ((int64_t)n + seg - 1) / seg;
+  return used < segments ? (int)used : segments;
 }
 
 __device__ __forceinline__ int fast_div(int x, uint32_t magic, uint32_t shift) {
