@@ -747,7 +747,7 @@ extern "C" int64_t qp_key_weights_workspace_size(const qp_key_weights_args *a) {
 extern "C" int qp_key_weights(const qp_key_weights_args *a, qp_stream_t stream) {
   const int st = check_key_weights(a);
   if (st != QP_OK) return st;
-  if (a->num_seqs == 0 || a->max_seqlen_k == 0) return QP_OK;
+  if (a->num_seqs == 0 || a->max_seqlen_k == 0 || a->max_blocks == 0) return QP_OK;  // (no position, or none with a page)
   QP_REQUIRE(a->key.codes && a->key.words && a->cu_seqlens_q && a->seqused_k && a->block_table && a->out,
              "qp_key_weights: null tensor");
   QP_REQUIRE(a->query || a->num_tokens == 0, "qp_key_weights: null tensor");
