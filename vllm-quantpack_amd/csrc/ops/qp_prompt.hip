@@ -20,6 +20,8 @@
 #include "qp_common.h"
 #include "quantpack_ops.h"
 
+#include <algorithm>
+
 namespace qp {
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -990,8 +992,10 @@ extern "C" int qp_prompt(const qp_prompt_args *a, qp_stream_t stream) {
   // In order of length against order of place, us: four turns of up to 509 tokens over up to 4605 keys, 32 / 8 heads of 64,
   // 48 / 61, of 128 72 / 88; prompts of up to 2048 tokens, heads of 128, 3 of them 67 / 71, 8 152 / 154 and 85 / 86; 12 of up
   // to 1500 105 / 104; 64 of up to 100 32 / 27.
+  // (Its products of keys and group, of 64 steps or of any sequence, stay below 2^31; max_seqlen_k may say less than there is.)
+  const int64_t longest = std::max({a->max_seqlen_k, a->num_keys, a->num_tokens, 64 * 64});
   const bool by_length = p.causal && splits == 1 && a->num_seqs > 1 && a->num_seqs <= 8 &&
-                         blocks * a->num_kv_heads > device_cus() && std::max(a->max_seqlen_k, a->num_tokens) * group < (1 << 29);
+                         blocks * a->num_kv_heads > device_cus() && longest * group < (1 << 29);
   p.step = by_length ? std::max(64, a->max_seqlen_k / 63) : 0;
   p.scale_log2 = a->softmax_scale * kLog2e;
   const int block_rows = prompt_rows(a);
