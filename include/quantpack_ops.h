@@ -65,6 +65,7 @@ int64_t qp_prompt_workspace_size(const qp_prompt_args *args);
  * token's own; the tokens of sequence i are its last cu_seqlens_q[i + 1] - cu_seqlens_q[i] positions. Entries from
  * seqused_k[i] on are left as they are. A token that sees no key adds nothing; a sequence without tokens keeps its
  * decayed weights. A key on a page outside 0 .. num_blocks - 1 is not seen and gets no weight.
+ * A query of NaN gives NaN to the keys that it sees, and nothing to the others.
  * out and previous may be the same tensor; with previous NULL, or decay 0, earlier weights are not read.
  */
 typedef struct qp_key_weights_args {

@@ -1,4 +1,4 @@
-"""key_weights where there is nothing to see."""
+"""key_weights where there is nothing to see, and where a query is no number."""
 import numpy as np
 import pytest
 
@@ -23,3 +23,31 @@ def test_weights_of_sequences_without_pages(device, tokens):
                     max_seqlen_q=tokens, softmax_scale=0.1, previous=torch.ones_like(out))
         torch.cuda.synchronize()
         assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("fmt,tokens", [("int4", 3), ("int8", 3), ("int4", 40), ("int8", 40)])
+@pytest.mark.parametrize("bad", [0, 1, -1])
+def test_weights_of_a_query_that_is_no_number(device, fmt, tokens, bad):
+    """A query of NaN gives NaN to the keys that it sees, and nothing to the others: keys after it, and pages that do not exist."""
+    import torch
+
+    from vllm_quantpack.attention.key_weights import key_weights
+    rng = np.random.default_rng(tokens)
+    hs, n, row = 128, 300, bad % tokens
+    kv, _ = random_cache(rng, 20, 2, 16, hs, fmt)
+    keep, (kc, _, ks, _) = torch_cache(kv, hs, fmt, device)
+    table = rng.permutation(20)[:19].astype(np.int32)
+    table[3] = -1
+    q = torch.randn((tokens, 4, hs), device=device).to(torch.bfloat16)
+    kw = dict(cu_seqlens_q=i32([0, tokens], device), seqused_k=i32([n], device), block_table=i32([table], device),
+              max_seqlen_q=tokens, softmax_scale=0.02)
+    want = key_weights(q, kc, ks, torch.zeros((1, 2, n), device=device), **kw)
+    q[row, 1] = float("nan")  # (a head of the first KV head)
+    got = key_weights(q, kc, ks, torch.zeros((1, 2, n), device=device), **kw)
+    torch.cuda.synchronize()
+    sees = n - tokens + row + 1
+    gone = torch.zeros(n, dtype=torch.bool, device=device)
+    gone[48:64] = True
+    assert bool((got[..., gone] == 0).all())
+    assert bool(got[0, 0, :sees][~gone[:sees]].isnan().all())
+    assert bool(got[0, 0, sees:].isfinite().all()) and torch.equal(got[0, 1], want[0, 1])

@@ -330,7 +330,8 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(const KeyWeightPar
       if (r0 + r >= nrows) break;
       const float2 st = stat[r0 + r];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) acc[i] = fmaf(__builtin_amdgcn_exp2f(x[r][i] - st.x), st.y, acc[i]);
+      for (int i = 0; i < kPer; ++i)  // (a key out of sight adds nothing, not even of a row whose sum is no number)
+        if (x[r][i] != -INFINITY) acc[i] = fmaf(__builtin_amdgcn_exp2f(x[r][i] - st.x), st.y, acc[i]);
     }
   }
 #pragma unroll
@@ -577,9 +578,9 @@ __global__ __launch_bounds__(kKwThreads, 2) void key_weights_kernel(const KeyWei
           for (int k = 0; k < kAt; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              float e = __builtin_amdgcn_exp2f(fmaf(d[k][4 * q + j], a[k], -mx[j]));
-              if (MASK && r0 + 8 * q + 4 * h + j < first_row[k]) e = 0.f;
-              sum[k] = fmaf(e, iv[j], sum[k]);
+              const float e = __builtin_amdgcn_exp2f(fmaf(d[k][4 * q + j], a[k], -mx[j]));
+              // (a row that does not see the key adds nothing, not even where its sum is no number)
+              if (!MASK || r0 + 8 * q + 4 * h + j >= first_row[k]) sum[k] = fmaf(e, iv[j], sum[k]);
             }
         }
       }
