@@ -238,6 +238,22 @@ def on_device_of(t: torch.Tensor):
     return _NO_GUARD if index == _current_device() else torch.cuda.device(index)
 
 
+_forward_ad = torch.autograd.forward_ad
+
+
+def no_derivatives(what: str, *tensors) -> None:
+    """NotImplementedError where a tensor (None: absent) carries a gradient or a tangent, which the call would drop.
+    (Forward-mode derivatives are taken under no_grad, too.)"""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"{what}: no backward pass; call it under torch.no_grad()")
+    if getattr(_forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what}: no forward-mode derivative; call it on the primal tensors")
+
+
 def same_device(what: str, first: torch.Tensor, **tensors) -> None:
     """ValueError unless first is on a GPU and every other tensor (None: absent) on the same one."""
     if not first.is_cuda:

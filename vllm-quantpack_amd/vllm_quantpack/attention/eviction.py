@@ -67,6 +67,7 @@ def evict_keys(k_cache, v_cache, k_scale_cache, v_scale_cache, weights, *, sequs
     _rows("new_weights", new_weights, torch.float32, seqs, nkv, budget)
     if new_seqused_k.dtype != torch.int32 or new_seqused_k.shape != (seqs,) or not new_seqused_k.is_contiguous():
         raise ValueError(f"evict_keys: new_seqused_k must be {seqs} contiguous int32 entries")
+    _hip.no_derivatives("evict_keys", weights, new_weights, k_scale_cache, v_scale_cache)
     table_at, new_table_at, used_at, new_used_at = (block_table.data_ptr(), new_block_table.data_ptr(), seqused_k.data_ptr(),
                                                     new_seqused_k.data_ptr())
     weights_at, new_weights_at = weights.data_ptr(), new_weights.data_ptr()

@@ -62,8 +62,7 @@ def key_weights(q, k_cache, k_scale_cache, out, *, cu_seqlens_q, seqused_k, bloc
     if query_signs is not None and (query_signs.dtype != torch.float32 or query_signs.shape != (hs,) or
                                     not query_signs.is_contiguous()):
         raise ValueError(f"key_weights: query_signs must be {hs} contiguous fp32 signs")
-    if torch.is_grad_enabled() and q.requires_grad:
-        raise NotImplementedError("key_weights: no backward pass; call it under torch.no_grad()")
+    _hip.no_derivatives("key_weights", q, k_scale_cache, out, previous, query_signs)
     index = q.get_device()
     if (index < 0 or not (index == k_cache.get_device() == k_scale_cache.get_device() == out.get_device() ==
                           cu_seqlens_q.get_device() == seqused_k.get_device() == block_table.get_device()) or

@@ -34,8 +34,7 @@ def _check(q, k, v, out, cu_q, cu_k, lse):
         raise ValueError("prompt_attention: cu_seqlens_q and cu_seqlens_k are of different batches")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2]):
         raise ValueError(f"prompt_attention: lse must be fp32 {tuple(q.shape[:2])}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise NotImplementedError("prompt_attention: no backward pass; call it under torch.no_grad()")
+    _hip.no_derivatives("prompt_attention", q, k, v, out, lse)
     index = q.get_device()
     if not (index == k.get_device() == v.get_device() == out.get_device() == cu_q.get_device() == cu_k.get_device()) or \
             index < 0 or (lse is not None and lse.get_device() != index):
