@@ -24,6 +24,7 @@ extern "C" {
  * cu_seqlens_q[num_seqs] are left as they are. Keys and values that no row sees may hold anything, NaN included.
  * When the rows alone cannot fill the GPU the keys are split over workgroups (num_splits, 0 = automatic) whose fp32
  * partials go to the workspace; an automatic choice without enough workspace falls back to one split.
+ * out may be query itself (the same address and strides); otherwise it shares no memory with query, key and value.
  */
 typedef struct qp_prompt_args {
   const void *query;           /* [num_tokens, num_q_heads, head_size], channels contiguous, rows 16-byte aligned */
@@ -66,7 +67,8 @@ int64_t qp_prompt_workspace_size(const qp_prompt_args *args);
  * seqused_k[i] on are left as they are. A token that sees no key adds nothing; a sequence without tokens keeps its
  * decayed weights. A key on a page outside 0 .. num_blocks - 1 is not seen and gets no weight.
  * A query of NaN gives NaN to the keys that it sees, and nothing to the others.
- * out and previous may be the same tensor; with previous NULL, or decay 0, earlier weights are not read.
+ * previous may be out itself (the same address and strides); otherwise the two share no memory. With previous NULL, or
+ * decay 0, earlier weights are not read.
  */
 typedef struct qp_key_weights_args {
   qp_cache_half key;
@@ -128,7 +130,8 @@ typedef struct qp_evict_args {
   int32_t budget;                 /* at least sinks + recent, and 1 */
   int32_t sinks;
   int32_t recent;
-  int32_t *kept;                  /* int32 [num_seqs, num_kv_heads, >= budget], contiguous in the last dimension */
+  int32_t *kept;                  /* int32 [num_seqs, num_kv_heads, >= budget], contiguous in the last dimension;
+                                     kept and new_weights share no memory with weights */
   int64_t kept_stride[2];
   float *new_weights;             /* fp32 [num_seqs, num_kv_heads, >= budget]; not the memory of weights */
   int64_t new_weights_stride[2];

@@ -12,7 +12,8 @@ import os
 import struct
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_void_p
 
-import torch  # noqa: F401  (must be loaded first: see module docstring)
+import numpy as np
+import torch  # noqa: F401  (must be loaded before the library: see module docstring)
 
 LIB_PATH = os.environ.get("QUANTPACK_HIP_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)),
                                                                  "libquantpack_hip.so")
@@ -244,14 +245,50 @@ _forward_ad = torch.autograd.forward_ad
 def no_derivatives(what: str, *tensors) -> None:
     """NotImplementedError where a tensor (None: absent) carries a gradient or a tangent, which the call would drop.
     (Forward-mode derivatives are taken under no_grad, too.)"""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise NotImplementedError(f"{what}: no backward pass; call it under torch.no_grad()")
-    if getattr(_forward_ad, "_current_level", 0) >= 0:
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"{what}: no backward pass; call it under torch.no_grad()")
+    if _forward_ad._current_level >= 0:
         for t in tensors:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{what}: no forward-mode derivative; call it on the primal tensors")
+
+
+def end_of(t: torch.Tensor, strides) -> int:
+    """The address past the last element of a 3-dimensional tensor."""
+    a, b, c = t.shape
+    return t.data_ptr() + ((a - 1) * strides[0] + (b - 1) * strides[1] + (c - 1) * strides[2] + 1) * t.element_size()
+
+
+def repeats(t: torch.Tensor, strides) -> bool:
+    """Whether t has the same elements again along a dimension, as expanded tensors do."""
+    return any(stride == 0 and size > 1 for size, stride in zip(t.shape, strides))
+
+
+class _Span:
+    """t's addresses as numpy sees them; never followed."""
+
+    def __init__(self, t):
+        size = t.element_size()
+        self.__array_interface__ = {"shape": tuple(t.shape), "typestr": f"|V{size}", "data": (t.data_ptr(), True),
+                                    "strides": tuple(x * size for x in t.stride()), "version": 3}
+
+
+def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether some element of a lies where one of b does, for 3-dimensional tensors whose extents meet."""
+    if not a.numel() or not b.numel():
+        return False
+    sa, sb = a.stride(), b.stride()
+    period = sa[0] * a.element_size()
+    if period > 0 and period == sb[0] * b.element_size():  # (views of one buffer's rows, side by side)
+        first, other = a.data_ptr(), b.data_ptr()
+        off = (other - first) % period
+        if end_of(a[:1], sa) - first <= off and off + end_of(b[:1], sb) - other <= period:
+            return False
+    try:  # (the general question takes 20 us)
+        return np.shares_memory(np.asarray(_Span(a)), np.asarray(_Span(b)), max_work=1 << 20)
+    except RuntimeError:  # (too hard to say: strides of no ordinary view)
+        return True
 
 
 def same_device(what: str, first: torch.Tensor, **tensors) -> None:

@@ -28,6 +28,13 @@ def _rows(name, t, dtype, seqs, nkv, length):
                          f"dimension, got {t.dtype} {tuple(t.shape)}")
 
 
+def _check_places(weights, written, name, length, budget):
+    """Places and weights are written while the weights are read, each by a workgroup of its own. (The two tensors' extents
+    meet.)"""
+    if _hip.share_memory(weights[..., :max(length, 0)], written[..., :max(budget, 0)]):
+        raise ValueError(f"evict_keys: weights are read while {name} are written: give other tensors")
+
+
 def evict_keys(k_cache, v_cache, k_scale_cache, v_scale_cache, weights, *, seqused_k, block_table, new_block_table, budget,
                max_seqlen_k=None, sinks=0, recent=0, kept=None, new_weights=None, new_seqused_k=None):
     """Keep min(seqused_k[i], budget) keys of every sequence i and KV head: the first `sinks`, the last `recent` and, of the
@@ -37,7 +44,8 @@ def evict_keys(k_cache, v_cache, k_scale_cache, v_scale_cache, weights, *, sequs
     The kept cells go to slots 0, 1, .. of new_block_table[i] (int32 [sequences, blocks], room for the budget, of blocks
     that no sequence of the call still uses), in the order of their positions. Returns (new_seqused_k int32 [sequences],
     kept int32 [sequences, NKV, budget] with the old positions, new_weights fp32 [sequences, NKV, budget] with their
-    weights), made when None, with -1 and 0 past a sequence's count; given ones are left as they are there.
+    weights), made when None, with -1 and 0 past a sequence's count; given ones are left as they are there. Given
+    ones share no memory with seqused_k and weights.
 
     No host synchronisation; the workspace comes from torch's caching allocator."""
     if k_cache.dim() != 4 or v_cache.dim() != 4 or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
@@ -70,11 +78,21 @@ def evict_keys(k_cache, v_cache, k_scale_cache, v_scale_cache, weights, *, sequs
     _hip.no_derivatives("evict_keys", weights, new_weights, k_scale_cache, v_scale_cache)
     table_at, new_table_at, used_at, new_used_at = (block_table.data_ptr(), new_block_table.data_ptr(), seqused_k.data_ptr(),
                                                     new_seqused_k.data_ptr())
-    weights_at, new_weights_at = weights.data_ptr(), new_weights.data_ptr()
     if seqs and block_table.numel() and new_table_at == table_at:
         raise ValueError("evict_keys: the kept cells move to other blocks: new_block_table must not be block_table")
-    if seqs and (new_weights_at == weights_at or new_used_at == used_at):
-        raise ValueError("evict_keys: weights and seqused_k are read while the new ones are written: give other tensors")
+    ws, ks, ns = weights.stride(), kept.stride(), new_weights.stride()
+    if (0 in ks and _hip.repeats(kept, ks)) or (0 in ns and _hip.repeats(new_weights, ns)):
+        raise ValueError("evict_keys: rows of kept or new_weights share memory with each other")
+    weights_at, kept_at, new_weights_at = weights.data_ptr(), kept.data_ptr(), new_weights.data_ptr()
+    if seqs:
+        end = weights_at + 4 * ((seqs - 1) * ws[0] + (nkv - 1) * ws[1] + weights.shape[2])
+        if kept_at < end and weights_at < kept_at + 4 * ((seqs - 1) * ks[0] + (nkv - 1) * ks[1] + kept.shape[2]):
+            _check_places(weights, kept, "kept", max_seqlen_k, budget)
+        if (new_weights_at < end and
+                weights_at < new_weights_at + 4 * ((seqs - 1) * ns[0] + (nkv - 1) * ns[1] + new_weights.shape[2])):
+            _check_places(weights, new_weights, "new_weights", max_seqlen_k, budget)
+    if seqs and new_used_at < used_at + 4 * seqs and used_at < new_used_at + 4 * seqs:
+        raise ValueError("evict_keys: seqused_k is read while the new one is written: give other tensors")
     index = k_cache.get_device()
     if index < 0 or not (index == v_cache.get_device() == k_scale_cache.get_device() == v_scale_cache.get_device() ==
                          weights.get_device() == seqused_k.get_device() == block_table.get_device() ==
@@ -84,11 +102,10 @@ def evict_keys(k_cache, v_cache, k_scale_cache, v_scale_cache, weights, *, sequs
                          weights=weights, seqused_k=seqused_k, block_table=block_table, new_block_table=new_block_table,
                          kept=kept, new_weights=new_weights, new_seqused_k=new_seqused_k)
     cache = _hip.paged_cache(k_cache, v_cache, k_scale_cache, v_scale_cache, hs)
-    ws, ks, ns = weights.stride(), kept.stride(), new_weights.stride()
     args = _hip.EvictArgs()
     _PACK.pack(args, weights_at, ws[0], ws[1], used_at, table_at, block_table.stride(0), new_table_at,
                new_block_table.stride(0), block_table.shape[1], new_block_table.shape[1], seqs, int(max_seqlen_k), budget,
-               sinks, recent, kept.data_ptr(), ks[0], ks[1], new_weights_at, ns[0], ns[1], new_used_at, 0, 0)
+               sinks, recent, kept_at, ks[0], ks[1], new_weights_at, ns[0], ns[1], new_used_at, 0, 0)
     lib = _hip.lib()
     with _hip.on_device_of(k_cache):
         need = lib.qp_evict_workspace_size(cache, args)

@@ -21,6 +21,17 @@ def _vector(name, t, length=None):
                          ("" if length is None else f" of {length} entries"))
 
 
+def _check_previous(previous, out, ps, os, length):
+    """Weights are written while others are read: previous lies in out's place, entry for entry, or apart from it."""
+    start, first = out.data_ptr(), previous.data_ptr()
+    if start >= _hip.end_of(previous, ps) or first >= _hip.end_of(out, os):
+        return
+    if first == start and all(n == 1 or x == y for n, x, y in zip(out.shape, ps, os)):
+        return
+    if _hip.share_memory(previous[..., :max(length, 0)], out[..., :max(length, 0)]):
+        raise ValueError("key_weights: previous shares memory with out but is not out")
+
+
 def key_weights(q, k_cache, k_scale_cache, out, *, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k=None,
                 softmax_scale, query_signs=None, previous=None, decay=1.0) -> torch.Tensor:
     """out[i, g, j] = decay * previous[i, g, j] + the sum over sequence i's query tokens and the query heads of KV head g of
@@ -29,9 +40,9 @@ def key_weights(q, k_cache, k_scale_cache, out, *, cu_seqlens_q, seqused_k, bloc
     q bf16 [T, NQ, hs] in the cache's domain, or unrotated with query_signs (`rht.signs`), which rotates each row as it
     loads; k_cache (blocks, bs, NKV, bytes) uint8 nibble pairs or int8 with its scale words k_scale_cache (the views of
     `k8v4_kv`; an int4 view's bytes past the codes are not read); out fp32 [sequences, NKV, L] with max_seqlen_k <= L (L
-    when None); previous: None, or weights of the same shape (out itself for an update in place). softmax_scale multiplies
-    q.k in the cache's domain, as in `prefill_attention`. A sequence's query tokens are the last of its positions and see
-    the keys up to their own; the first max_seqlen_q of them are counted.
+    when None); previous: None, or weights of the same shape (out itself for an update in place, else apart from it).
+    softmax_scale multiplies q.k in the cache's domain, as in `prefill_attention`. A sequence's query tokens are the last of
+    its positions and see the keys up to their own; the first max_seqlen_q of them are counted.
 
     A token that sees no key adds nothing, a sequence without tokens keeps its decayed weights, and a key on a page outside
     the cache gets none. The workspace comes from torch's caching allocator; no host synchronisation."""
@@ -55,6 +66,12 @@ def key_weights(q, k_cache, k_scale_cache, out, *, cu_seqlens_q, seqused_k, bloc
         max_seqlen_k = out.shape[2]
     if max_seqlen_k > out.shape[2]:
         raise ValueError(f"key_weights: out has {out.shape[2]} positions, the longest context {max_seqlen_k}")
+    os = out.stride()
+    if 0 in os and _hip.repeats(out, os):
+        raise ValueError("key_weights: rows of out share memory with each other")
+    ps = (0, 0) if previous is None else previous.stride()
+    if previous is not None and decay and (ps != os or previous.data_ptr() != out.data_ptr()):
+        _check_previous(previous, out, ps, os, max_seqlen_k)
     _vector("seqused_k", seqused_k)
     _vector("cu_seqlens_q", cu_seqlens_q, seqs + 1)
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != seqs or block_table.stride(1) != 1:
@@ -72,8 +89,7 @@ def key_weights(q, k_cache, k_scale_cache, out, *, cu_seqlens_q, seqused_k, bloc
                          seqused_k=seqused_k, block_table=block_table, query_signs=query_signs, previous=previous)
     if k_scale_cache.dtype not in _hip._WORD_DTYPES:
         raise ValueError(f"key_weights: scale words must be 4-byte elements, got {k_scale_cache.dtype}")
-    cs, ws, qs, os = k_cache.stride(), k_scale_cache.stride(), q.stride(), out.stride()
-    ps = (0, 0) if previous is None else previous.stride()
+    cs, ws, qs = k_cache.stride(), k_scale_cache.stride(), q.stride()
     args = _hip.KeyWeightsArgs()
     _PACK.pack(args, k_cache.data_ptr(), cs[0], cs[1], cs[2], k_scale_cache.data_ptr(), ws[0], ws[1], ws[2],
                _hip.CODES_INT8 if k_cache.dtype == torch.int8 else _hip.CODES_INT4, k_cache.shape[0], k_cache.shape[1], nkv,

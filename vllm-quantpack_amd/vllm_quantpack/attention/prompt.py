@@ -17,7 +17,7 @@ _PACK = _hip.Packer(_hip.PromptArgs)
 
 
 def _check(q, k, v, out, cu_q, cu_k, lse):
-    """What the kernel's indexing rests on (shapes, types and places; nothing is copied)."""
+    """What the kernel's indexing rests on (shapes and types; nothing is copied)."""
     if q.dtype not in _DTYPES:
         raise NotImplementedError(f"prompt_attention: bf16 or fp16 tensors, got {q.dtype}")
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2] or out.shape != q.shape:
@@ -35,6 +35,22 @@ def _check(q, k, v, out, cu_q, cu_k, lse):
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2]):
         raise ValueError(f"prompt_attention: lse must be fp32 {tuple(q.shape[:2])}")
     _hip.no_derivatives("prompt_attention", q, k, v, out, lse)
+
+
+def _check_out(q, k, v, out):
+    """Row blocks are written while others are at work: out lies in q's place, row for row, or apart from all three. (Their
+    extents meet, or out has a stride of 0.)"""
+    if _hip.repeats(out, out.stride()):
+        raise ValueError("prompt_attention: rows of out share memory with each other")
+    same = out.data_ptr() == q.data_ptr() and all(n == 1 or x == y for n, x, y in zip(q.shape, q.stride(), out.stride()))
+    if not same and _hip.share_memory(out, q):
+        raise ValueError("prompt_attention: out shares memory with q but is not q")
+    for name, t in (("k", k), ("v", v)):
+        if _hip.share_memory(out, t):
+            raise ValueError(f"prompt_attention: out shares memory with {name}")
+
+
+def _check_device(q, k, v, out, cu_q, cu_k, lse):
     index = q.get_device()
     if not (index == k.get_device() == v.get_device() == out.get_device() == cu_q.get_device() == cu_k.get_device()) or \
             index < 0 or (lse is not None and lse.get_device() != index):
@@ -48,9 +64,10 @@ def prompt_attention(q, k, v, out=None, *, cu_seqlens_q, cu_seqlens_k=None, max_
     of k and v (int32 on the GPU; cu_seqlens_k None: the same as the queries'). Its last query is at its last key: with
     causal, query t sees the keys j <= t + keys - queries. softmax_scale (hs ** -0.5 when None) multiplies q.k.
 
-    Writes and returns out (made when None); a query that sees no key gets zeros. lse (optional, fp32 [T, NQ]) receives
-    the natural-log sum of the row's exponentials, -inf for such a query. Rows of q past the last sequence are not
-    written. Keys and values that no query sees are never used, whatever they hold.
+    Writes and returns out (made when None; it may be q itself, else it shares no memory with q, k and v); a query that
+    sees no key gets zeros. lse (optional, fp32 [T, NQ]) receives the natural-log sum of the row's exponentials, -inf for
+    such a query. Rows of q past the last sequence are not written. Keys and values that no query sees are never used,
+    whatever they hold.
 
     Strides are free as long as channels are contiguous and rows 16-byte aligned, so q, k and v may be views of one
     projection's output. max_seqlen_k, the longest sequence's keys (K when None), is what the work is laid out by: the
@@ -59,18 +76,30 @@ def prompt_attention(q, k, v, out=None, *, cu_seqlens_q, cu_seqlens_k=None, max_
     del max_seqlen_q
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens_q
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     _check(q, k, v, out, cu_seqlens_q, cu_seqlens_k, lse)
     hs = q.shape[2]
     qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
     ls = (0, 0) if lse is None else lse.stride()
+    if lse is not None and 0 in ls and _hip.repeats(lse, ls):
+        raise ValueError("prompt_attention: lse must have a place for every row")
+    q_at, k_at, v_at, out_at = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    if given:
+        (T, nq, _), (K, nkv, _) = q.shape, k.shape
+        end = out_at + 2 * ((T - 1) * os[0] + (nq - 1) * os[1] + hs)
+        if (0 in os or (out_at < q_at + 2 * ((T - 1) * qs[0] + (nq - 1) * qs[1] + hs) and q_at < end) or
+                (out_at < k_at + 2 * ((K - 1) * ks[0] + (nkv - 1) * ks[1] + hs) and k_at < end) or
+                (out_at < v_at + 2 * ((K - 1) * vs[0] + (nkv - 1) * vs[1] + hs) and v_at < end)):
+            _check_out(q, k, v, out)
+    _check_device(q, k, v, out, cu_seqlens_q, cu_seqlens_k, lse)
     args = _hip.PromptArgs()
-    _PACK.pack(args, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+    _PACK.pack(args, q_at, qs[0], qs[1], k_at, ks[0], ks[1], v_at, vs[0], vs[1],
                cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), cu_seqlens_q.shape[0] - 1, q.shape[0], k.shape[0],
                q.shape[1], k.shape[1], hs, _DTYPES[q.dtype],
                int(k.shape[0] if max_seqlen_k is None else min(max_seqlen_k, k.shape[0])), int(num_splits), int(causal),
-               float(hs ** -0.5 if softmax_scale is None else softmax_scale), out.data_ptr(), os[0], os[1],
+               float(hs ** -0.5 if softmax_scale is None else softmax_scale), out_at, os[0], os[1],
                0 if lse is None else lse.data_ptr(), ls[0], ls[1], 0, 0)
     lib = _hip.lib()
     with _hip.on_device_of(q):
