@@ -103,6 +103,7 @@ def draw(rng):
         budget = max(8, int(context * rng.uniform(0.05, 0.8)))
         c = evict("", rng.choice(("int4", "int4", "int8")), nkv, hs, seqs, context, budget, rng.choice((0, 1, 4, 7)),
                   min(budget // 2, rng.choice((0, 8, 33, 128))), rng.choice((16, 16, 32, 48)), ragged, lens)
+        c["sinks"] = min(c["sinks"], budget - c["recent"])  # (a budget holds both)
     del c["name"]
     return c
 
