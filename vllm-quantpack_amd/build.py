@@ -33,7 +33,8 @@ def hipcc():
 
 
 # Per-source extra flags. The prefill kernel keeps its QK^T MFMA results in VGPRs (its PV accumulators own the AGPRs);
-# the dual prefill kernel and those of csrc/ops keep all of them there (256 VGPRs per wave, no AGPRs).
+# the dual prefill kernel and those of csrc/ops keep all MFMA results there (256 registers per wave; prompt_attention at
+# heads 256 and 512, where a wave has a SIMD for itself, 499 and 393).
 # The decode kernels take no NaN inputs (masked scores are -inf, never NaN), so their maxima need no quieting.
 EXTRA = {"qp_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
          "qp_prefill_dual.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],

@@ -8,10 +8,11 @@
 // Every weight has one owner, so no order of additions varies. With few query rows (a decode step) the scores are made once
 // and kept between the passes; with many (the last tokens of a prompt) they are made twice, from keys unpacked in registers.
 //
-// What bounds it, measured: one token, 24 / 4 heads of 256, over 131072 int4 keys takes 31 us for the scores and 9.5 for the
-// sums. A cell's key half lies beside its value half, so that nearly all lines of the cache are fetched: 138 MB for 66 of key
-// codes, at 4.45 TB/s. 64 tokens over 32768 keys, 64 / 8 heads of 128: 62 us for the statistics and 50 for the weights, 550
-// and 690 TFLOP/s, exponentials and products taking about as long, and 10 for rows and statistics.
+// What bounds it, measured: one token, 24 / 4 heads of 256, over 131072 int4 keys takes 30 us for the scores and 9.7 for the
+// sums. A cell's key half lies beside its value half, so that nearly all lines of the cache are fetched: 135 MB for 66 of key
+// codes, at 4.5 TB/s. 64 tokens over 32768 keys, 64 / 8 heads of 128: 62 us for the statistics and 49 for the weights, 550
+// and 700 TFLOP/s, and 10 for rows and statistics. In the two passes the matrix pipes are busy for 33 and 38 % of the cycles and
+// the vector pipes for 65 and 56: exponentials and scaling run beside the products only in part.
 //
 // Precision: codes enter the product as code - 8 (int4) or as they are (int8), exact in bf16 and centred, so that the zero
 // point's share, sum(q) (zp - 8), takes away little; scores meet the row's maximum in one fused multiply-add.
@@ -496,7 +497,7 @@ __global__ __launch_bounds__(kKwThreads, 2) void key_weights_kernel(const KeyWei
       kz[k] = zero_operand(word_zero<FMT>(word[k]), h);
 #pragma unroll
       for (int i = 0; i < Sh::kSteps; ++i) kop[k][i] = key_operand<HS, FMT>(raw[k], i);
-      // (a key that is not there has the scale NaN, which no stored one has)
+      // (a key that is not there has the scale NaN, which the store never writes: its scales are at least 1e-6)
       if (PASS == 1 && h == 0) kscale[w][32 * k + col] = ok[k] ? a[k] : __builtin_nanf("");
       sum[k] = 0.f;
       first_row[k] = max(0, kw + 32 * k + col - before) * G;

@@ -12,11 +12,11 @@
 // and the packed probabilities are the B operand of the second product as they are. K and V tiles are copied to LDS as they
 // lie in memory, a tile ahead of their use; the V^T operand comes from the LDS's transposing reads (ds_read_b64_tr_b16).
 //
-// What bounds it, measured: 16384 tokens, 32 / 8 heads of 128, take 1.97 ms = 1110 TFLOP/s. MFMAs keep the matrix pipes busy
-// for 56 % of the cycles at 1.9 GHz and the softmax the vector pipes for 53 %; the same kernel's MFMAs alone take 1.61 ms,
-// without the exponentials it takes 1.87, without the reads of K and V from LDS 1.84. A token over 65536 keys, 64 / 8 heads:
-// 57 us for the walk = 4.7 TB/s, and 4.7 for the merge. Small batches are bound by the blocks with the most keys and by each
-// block's start, 3 to 4 us.
+// What bounds it, measured: 16384 tokens, 32 / 8 heads of 128, take 1.94 to 2.02 ms = 1090 to 1130 TFLOP/s. MFMAs keep the
+// matrix pipes busy for 57 % of the cycles at 1.9 GHz and the vector pipes are busy for 54 %; the same kernel's MFMAs alone take
+// 1.61 ms, without the exponentials it takes 1.87, without the reads of K and V from LDS 1.84. At head 256 (4096 tokens, 24 / 4
+// heads, 257 us) the two are busy for 33 and 28 %. A token over 65536 keys, 64 / 8 heads of 128: 57 us for the walk = 4.7 TB/s,
+// and 4.9 for the merge. Small batches are bound by the blocks with the most keys and by each block's start, 3 to 4 us.
 #include "qp_common.h"
 #include "quantpack_ops.h"
 
@@ -63,7 +63,7 @@ constexpr float kPromptNone = -1e30f;  // a row's reference before it has seen a
 // and the row's sum above 2^below. bf16 has the exponents of fp32. fp16 loses bits below 2^-14 and has nothing below 2^-25, while
 // the sum takes unrounded probabilities: with the largest at 2^7 or more, and at most 2^15, a key loses 2^-32 of the sum at
 // most. Relative to the maximum itself, 65536 keys 17 nats below another's came out 43 % wrong, and 18 nats below as nothing; a
-// call takes up to 1 % longer.
+// call takes up to 1.3 % longer.
 template <bool F16>
 constexpr float prompt_below = F16 ? 7.f : 0.f;
 constexpr float kPromptHeadroom = 8.f;

@@ -248,7 +248,7 @@ def no_derivatives(what: str, *tensors) -> None:
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError(f"{what}: no backward pass; call it under torch.no_grad()")
-    if _forward_ad._current_level >= 0:
+    if getattr(_forward_ad, "_current_level", 0) >= 0:
         for t in tensors:
             if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{what}: no forward-mode derivative; call it on the primal tensors")
